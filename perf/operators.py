@@ -166,6 +166,13 @@ def prepare(case, seed):
         s.update(add=torch.tensor(add, device=dev, dtype=torch.int32), kv_len=torch.tensor(lens, device=dev, dtype=torch.int32),
                  table=table, ring=ring, counters=torch.tensor([head, head + tail], device=dev, dtype=torch.int64),
                  page=case["page"], room=case["room"])
+        # the buffers that a step's plan lives in, kept by the serving loop
+        R, T = case["rows"], case["room"]
+        i32 = dict(device=dev, dtype=torch.int32)
+        s["out"] = dict(cu=torch.empty(R + 1, **i32), row=torch.empty(T, **i32), pos=torch.empty(T, **i32),
+                        slot=torch.empty(T, device=dev, dtype=torch.int64),
+                        unit=torch.empty(min(T, T // case["page"] + 2 * R), 4, **i32), kv_len=torch.empty(R, **i32),
+                        counters=torch.empty(2, device=dev, dtype=torch.int64), info=torch.empty(4, **i32))
         return s
     if case["op"] == "append":
         H, Hkv, D, P, T, R = (case[k] for k in ("heads", "kv_heads", "dim", "page", "tokens", "rows"))
@@ -433,9 +440,9 @@ def run(s):
         return {"attn": _attn_plain, "gather": _gather_plain, "sample": _sample_plain}[op](s)
     from hetero_cp_ringattn_b200.ops import paged, sampling
     if op == "plan":
-        p = paged.plan_step(s["add"], s["kv_len"], s["table"], s["ring"], s["counters"], page=s["page"], max_tokens=s["room"])
-        return {"cu": p.cu, "row": p.row, "pos": p.pos, "slot": p.slot, "unit": p.unit, "kv_len": p.kv_len,
-                "counters": p.counters, "info": p.info, "table": s["table"], "ring": s["ring"]}
+        paged.plan_step(s["add"], s["kv_len"], s["table"], s["ring"], s["counters"], page=s["page"], max_tokens=s["room"],
+                        out=paged.StepPlan(**s["out"]))
+        return {**s["out"], "table": s["table"], "ring": s["ring"]}
     if op == "append":
         c = s["case"]
         q = paged.rope_append_kv8(s["qkv"], s["cos"], s["sin"], s["pos"], s["units"], s["table"], s["k"], s["v"], s["k_scale"],

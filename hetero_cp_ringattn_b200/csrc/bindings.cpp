@@ -769,7 +769,11 @@ class PyRuntime {
 
 }  // namespace
 
+// the paged 8-bit cache and the sampler (bindings_paged.cpp)
+void bind_paged(py::module& m);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  bind_paged(m);
   m.doc() = "hetero_cp_ringattn_b200 sm_100a kernels and domain runtime";
   m.def("gemm", &gemm, "tcgen05 GEMM with fused epilogue", py::arg("A"), py::arg("B"), py::arg("C"),
         py::arg("epi") = 0, py::arg("bias") = py::none(), py::arg("R") = py::none(),

@@ -29,11 +29,16 @@ NVCC_FLAGS = ARCH + DEBUG + ["-O3", "-std=c++17", "-lineinfo", "--use_fast_math"
                      "--expt-relaxed-constexpr"]
 SOURCES = [
     "bindings.cpp",
+    "bindings_paged.cpp",
     "core/runtime.cu",
     "kernels/gemm_sm100.cu",
     "kernels/attn_fwd_sm100.cu",
     "kernels/elementwise.cu",
     "kernels/decode.cu",
+    "kernels/plan_step.cu",
+    "kernels/kv8_cache.cu",
+    "kernels/kv8_attn.cu",
+    "kernels/sample.cu",
 ]
 
 # host runtime library (no CUDA, no libtorch): layouts, capacity, schedule, pages, scheduler

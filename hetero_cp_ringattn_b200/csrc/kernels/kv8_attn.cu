@@ -41,30 +41,62 @@ constexpr int kTile = 32;     // cached tokens a tile
 constexpr float kShift = 15.f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-template <int D>
-struct Ring {
-  static constexpr int kBytes = 2 * kTile * D;            // K and V of a tile
-  static constexpr int kStages = D == 128 ? 3 : 6;        // 192 KB for the 8 warps
+// How the warps of a CTA share a tile stream. Up to 16 query rows (NT <= 2 column tiles): a stream a
+// warp. More (NT = 3 or 5): two warps a stream, which split the tile's tokens in the scores and the
+// head dims in O, so that up to 40 rows take one pass over the cache with their accumulators in
+// registers and no code is converted twice.
+template <int D, int NT>
+struct Shape {
+  static constexpr bool kPair = NT > 2;
+  static constexpr int kRows = 8 * NT;                      // query rows of an item
+  static constexpr int kStreams = kPair ? kWarps / 2 : kWarps;
+  static constexpr int kBytes = 2 * kTile * D;              // K and V of a tile
+  static constexpr int kStages = 196608 / (kStreams * kBytes);   // 192 KB of rings: 3 to 12 stages
+  static constexpr int kRing = kStages * kBytes;
+  static_assert(kRing >= kRows * D * 4, "a stream's last piece is left in its ring");
 };
 
-struct Layout {  // workspace
-  long long* prefix;   // [B + 1] tiles before each request
-  float* ml;           // [workers][2][rows][2]
-  float* o;            // [workers][2][rows][D]
+// An item (request, KV head, query row tile) that goes on in the next CTA.
+struct Straddle {
+  int b, h, rt;
+  int last;            // the last CTA that works on it; -1: none
+};
+
+struct Workspace {
+  Straddle* straddle;  // [CTAs]
+  float* ml;           // [CTAs][2][rows][2]   piece 0: of the item at the range's start; 1: at its end
+  float* o;            // [CTAs][2][rows][D]
+  float* head;         // [CTAs][streams][rows][D]  first pieces of streams that go on with another item
+  size_t bytes;
 };
 
 __host__ __device__ inline size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 
-__host__ __device__ inline Layout layout_of(void* ws, int B, int workers, int rows) {
+__host__ __device__ inline Workspace workspace_of(void* ws, int ctas, int streams, int rows, int D) {
   char* p = reinterpret_cast<char*>(ws);
-  Layout l;
-  l.prefix = reinterpret_cast<long long*>(p);
-  p += align256(size_t(B + 1) * sizeof(long long));
-  l.ml = reinterpret_cast<float*>(p);
-  p += align256(size_t(workers) * 2 * rows * 2 * sizeof(float));
-  l.o = reinterpret_cast<float*>(p);
-  return l;
+  Workspace w;
+  w.straddle = reinterpret_cast<Straddle*>(p);
+  size_t at = align256(size_t(ctas) * sizeof(Straddle));
+  w.ml = reinterpret_cast<float*>(p + at);
+  at += align256(size_t(ctas) * 2 * rows * 2 * sizeof(float));
+  w.o = reinterpret_cast<float*>(p + at);
+  at += align256(size_t(ctas) * 2 * rows * D * sizeof(float));
+  w.head = reinterpret_cast<float*>(p + at);
+  at += align256(size_t(ctas) * streams * rows * D * sizeof(float));
+  w.bytes = at;
+  return w;
 }
+
+// The tile list in `n` equal ranges: part i starts at begin(i).
+struct Split {
+  long long q, r;
+  __device__ __forceinline__ Split(long long total, int n) : q(total / n), r(total % n) {}
+  __device__ __forceinline__ long long begin(int i) const { return q * i + min((long long)i, r); }
+  __device__ __forceinline__ int part_of(long long x) const {   // the part that holds x
+    const long long big = r * (q + 1);
+    return int(x < big ? x / (q + 1) : r + (x - big) / q);
+  }
+};
 
 __device__ __forceinline__ void tma_load_4d(void* dst, const void* map, uint64_t* bar, int c1, int c2, int c3) {
   asm volatile(
@@ -128,33 +160,49 @@ __device__ __forceinline__ int rows_of(const AttnArgs& a, int b) {
   return int(min((long long)max(a.kv_len[b], 0), (long long)a.width * a.c.P));
 }
 
-// One warp's place in the tile list.
+// A place in the tile list.
 struct Place {
   int b, h, rt, tile, tiles;  // request, KV head, query row tile, tile and tiles of the item
+  int n, qn, first;           // the request's cached rows, query tokens and the first of them
 };
 
-// First worker whose range [w W / NW, (w + 1) W / NW) reaches past x.
-__device__ __forceinline__ int worker_of(long long x, long long W, int NW) { return int(((x + 1) * NW - 1) / W); }
+// A finished row: o = acc / l, lse = (m - 15 + log2 l) ln 2; l = 0: the row saw nothing.
+__device__ __forceinline__ float row_lse(float m, float l) { return l == 0.f ? -INFINITY : (m - kShift + log2f(l)) * kLn2; }
+__device__ __forceinline__ float row_inv(float l) { return l == 0.f ? 0.f : __frcp_rn(l); }
+
+__device__ __forceinline__ void pair_sync(int pair) { asm volatile("bar.sync %0, 64;" ::"r"(pair + 1) : "memory"); }
 
 template <int D, int NT, bool INT8>
 __global__ void __launch_bounds__(kWarps * 32, 1)
 attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, AttnArgs a) {
-  constexpr int kStages = Ring<D>::kStages, kBytes = Ring<D>::kBytes, kChunks = D / 16, kRows = 8 * NT;
+  using S = Shape<D, NT>;
+  constexpr bool kPair = S::kPair;
+  constexpr int kStages = S::kStages, kBytes = S::kBytes, kRows = S::kRows, kStreams = S::kStreams;
+  constexpr int kChunks = D / 16;                          // 16-dim pieces of a row
+  constexpr int kMt = kPair ? 1 : 2;                       // 16-token groups whose scores a warp computes
+  constexpr int kOut = kPair ? kChunks / 2 : kChunks;      // pieces of O a warp accumulates
   extern __shared__ unsigned char raw[];
   unsigned char* ring_base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  long long* prefix = reinterpret_cast<long long*>(ring_base + kWarps * kStages * kBytes);
-  __shared__ uint64_t bars[kWarps][kStages];
-  __shared__ float meta[kWarps][kStages][4];   // k scale and v scale of the tile's two halves
+  long long* prefix = reinterpret_cast<long long*>(ring_base + kStreams * S::kRing);
+  __shared__ uint64_t bars[kStreams][kStages];
+  __shared__ float meta[kStreams][kStages][4];             // k scale and v scale of the tile's two halves
   __shared__ long long warp_tot[kWarps];
+  __shared__ float s_ml[kStreams][2][kRows][2];            // (m, l) of the streams' pieces
+  __shared__ long long s_start[kStreams][2];               // first tile of the piece's item; -1: no piece
+  __shared__ Place s_place[kStreams][2];
+  __shared__ float s_max[kPair ? kStreams : 1][2][kRows];  // pair: column maxima of the two warps
+  __shared__ uint32_t s_p[kPair ? kStreams : 1][2][kPair ? NT * 2 : 1][32];   // pair: their P^T fragments
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int stream = kPair ? warp >> 1 : warp, sub = kPair ? warp & 1 : 0;
   const int G = a.H / a.c.Hkv, P = a.c.P, Hkv = a.c.Hkv;
   if (tid == 0) {
-    for (int w = 0; w < kWarps; ++w)
+    for (int w = 0; w < kStreams; ++w)
       for (int i = 0; i < kStages; ++i) mbar_init(&bars[w][i], 1);
     fence_barrier_init();
     tma_prefetch_desc(&kmap);
     tma_prefetch_desc(&vmap);
   }
+  if (tid < kStreams * 2) s_start[tid >> 1][tid & 1] = -1;
   pdl_trigger();
   pdl_wait();
 
@@ -186,13 +234,11 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
     }
     __syncthreads();
   }
-  const int NW = gridDim.x * kWarps, worker = warp * gridDim.x + blockIdx.x;
-  const Layout L = layout_of(a.workspace, a.B, NW, kRows);
-  if (blockIdx.x == 0)
-    for (int b = tid; b <= a.B; b += kWarps * 32) L.prefix[b] = prefix[b];
   const long long W = prefix[a.B];
-  const long long x0 = W * worker / NW, x1 = W * (worker + 1) / NW;
-  if (x0 >= x1) return;
+  const Split ctas(W, gridDim.x);
+  const long long c0 = ctas.begin(blockIdx.x), c1 = ctas.begin(blockIdx.x + 1);
+  const long long x0 = c0 + (c1 - c0) * stream / kStreams, x1 = c0 + (c1 - c0) * (stream + 1) / kStreams;
+  const Workspace ws = workspace_of(a.workspace, gridDim.x, kStreams, kRows, D);
 
   auto place_of = [&](long long x) {
     int lo = 0, hi = a.B;
@@ -203,9 +249,10 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
     }
     Place p;
     p.b = lo;
-    int first;
-    const int rts = (q_tokens(a, lo, first) * G + kRows - 1) / kRows;
-    p.tiles = (rows_of(a, lo) + kTile - 1) / kTile;
+    p.qn = q_tokens(a, lo, p.first);
+    p.n = rows_of(a, lo);
+    const int rts = (p.qn * G + kRows - 1) / kRows;
+    p.tiles = (p.n + kTile - 1) / kTile;
     const long long rem = x - prefix[lo];
     const int item = int(rem / p.tiles);
     p.tile = int(rem - (long long)item * p.tiles);
@@ -214,20 +261,20 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
     return p;
   };
 
-  // ---------------------------------------------------------------- the copies' side
-  unsigned char* ring = ring_base + warp * kStages * kBytes;
+  // ---------------------------------------------------------------- the copies' side (one warp a stream)
+  unsigned char* ring = ring_base + stream * S::kRing;
   // a tile lies in one page of 32 tokens or more, or in two of 16 (lane 1 brings the second half)
   const int halves = P == 16 ? 2 : 1;
   const int box = min(P, kTile);
   long long px = x0;          // next tile whose page is looked up
-  Place pp = place_of(px);
+  Place pp{};
   int next_page = -1, next_row = 0, next_h = 0;   // looked up, not yet copied
   bool next_valid = false;
   auto look_up = [&] {
     next_valid = false;
     if (px < x1) {
       const int block = pp.tile * kTile / P + lane;
-      if (lane < halves && block * P < rows_of(a, pp.b)) {
+      if (lane < halves && block * P < pp.n) {
         next_page = a.table[(long)pp.b * a.width + block];
         next_valid = true;
       }
@@ -241,11 +288,11 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
   int load_stage = -1;
   auto put_scales = [&] {
     if (load_stage >= 0 && lane < halves) {
-      meta[warp][load_stage][2 * lane] = load_ks;
-      meta[warp][load_stage][2 * lane + 1] = load_vs;
+      meta[stream][load_stage][2 * lane] = load_ks;
+      meta[stream][load_stage][2 * lane + 1] = load_vs;
       if (halves == 1) {
-        meta[warp][load_stage][2] = load_ks;
-        meta[warp][load_stage][3] = load_vs;
+        meta[stream][load_stage][2] = load_ks;
+        meta[stream][load_stage][3] = load_vs;
       }
     }
     load_stage = -1;
@@ -253,7 +300,7 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
   auto copy = [&](int stage) {
     const uint32_t valid = __ballot_sync(0xffffffffu, next_valid);
     if (valid == 0) return;
-    uint64_t* bar = &bars[warp][stage];
+    uint64_t* bar = &bars[stream][stage];
     if (lane == 0) mbar_arrive_expect_tx(bar, uint32_t(__popc(valid)) * 2u * uint32_t(box) * D);
     __syncwarp();
     load_ks = load_vs = 1.f;
@@ -272,27 +319,33 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
     }
     load_stage = stage;
   };
-  look_up();
-#pragma unroll 1
-  for (int i = 0; i < kStages; ++i) {
-    put_scales();
-    copy(i);
+  const bool copies = sub == 0;
+  if (copies && x0 < x1) {
+    pp = place_of(px);
     look_up();
+#pragma unroll 1
+    for (int i = 0; i < kStages; ++i) {
+      put_scales();
+      copy(i);
+      look_up();
+    }
+    put_scales();
   }
-  put_scales();
-  __syncwarp();
+  if (kPair) pair_sync(stream);
+  else __syncwarp();
 
   // ---------------------------------------------------------------- the products' side
   const int j = lane >> 2, c = lane & 3;   // fragment row and column group of the lane
-  int stage = 0;
+  const int out0 = sub * kOut;             // first piece of O of this warp
+  int stage = 0, spent = -1;               // spent: pair mode, the stage both warps are done with
   uint32_t phase = 0;
   long long x = x0;
+  // A wait that ran out (reported) ends the waiting and the copies, not the loop: the barriers that two
+  // warps share stay matched, and the rest of the range is computed on whatever the ring holds.
   bool alive = true;
-  while (x < x1 && alive) {
+  while (x < x1) {
     const Place p = place_of(x);
-    const int n = rows_of(a, p.b);
-    int first;
-    const int qn = q_tokens(a, p.b, first);
+    const int n = p.n, qn = p.qn;
     const int end = int(min((long long)p.tiles, p.tile + (x1 - x)));
     const int r0 = p.rt * kRows, rows = min(qn * G - r0, kRows);   // the item's query rows
 
@@ -302,7 +355,7 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
     float f[NT][2];          // score factor of the lane's two columns
     int lim[NT][2];          // rows seen by them
     float m[NT][2], l[NT][2];
-    float acc[kChunks][NT][4];
+    float acc[kOut][NT][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int r = t * 8 + j;
@@ -310,7 +363,7 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
       float top = 0.f;
       const bool have = r < rows;
       const int qi = (r0 + r) / G, g = (r0 + r) % G;
-      const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (long)(first + qi) * a.q_stride +
+      const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (long)(p.first + qi) * a.q_stride +
                             (long)(p.h * G + g) * a.q_head_stride + 4 * c;
 #pragma unroll
       for (int s = 0; s < kChunks; ++s) {
@@ -326,7 +379,7 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // |q| 2^k in [2^14, 2^15) for the row's largest element
+      // |q| 2^e in [2^14, 2^15) for the row's largest element
       const int e = top > 0.f ? max(-113, min(100, 14 - (((__float_as_int(top) >> 23) & 0xff) - 127))) : 0;
       const float up = pow2(e);
 #pragma unroll
@@ -344,7 +397,7 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
         l[t][i] = 0.f;
       }
 #pragma unroll
-      for (int s = 0; s < kChunks; ++s)
+      for (int s = 0; s < kOut; ++s)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[s][t][i] = 0.f;
     }
@@ -352,20 +405,21 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
     const int least = n - qn + qi0 + 1;                   // rows that all of them see
 
     for (int tile = p.tile; tile < end; ++tile, ++x) {
-      if (!mbar_wait(&bars[warp][stage], phase, a.status, 412)) {
-        alive = false;
-        break;
-      }
+      if (alive) alive = mbar_wait(&bars[stream][stage], phase, a.status, 412);
       const int base = tile * kTile;
       const uint32_t kbase = smem_u32(ring + stage * kBytes), vbase = kbase + kTile * D;
-      // ---- S^T = K Q^T
-      float s[2][NT][4];
+      const bool edge = base + kTile > least;
+      // ---- S^T = K Q^T, in the log2 domain, masked
+      float s[kMt][NT][4];
+      float iv[kMt];
+      bool dead[kMt];
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
+      for (int mi = 0; mi < kMt; ++mi) {
+        const int mt = kPair ? sub : mi;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[mt][t][i] = 0.f;
+          for (int i = 0; i < 4; ++i) s[mi][t][i] = 0.f;
 #pragma unroll
         for (int k = 0; k < kChunks; k += 2) {
           uint32_t r[4];
@@ -376,40 +430,63 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
             decode4<INT8>(r[2 * h], af[0], af[2]);
             decode4<INT8>(r[2 * h + 1], af[1], af[3]);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) mma_f16(s[mt][t], af, qf[t][k + h][0], qf[t][k + h][1]);
+            for (int t = 0; t < NT; ++t) mma_f16(s[mi][t], af, qf[t][k + h][0], qf[t][k + h][1]);
           }
         }
-      }
-      // ---- scores in the log2 domain, masked, and the running maximum
-      const bool edge = base + kTile > least;
-      float lv[2], iv[2];
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        const float ks = meta[warp][stage][2 * mt], vs = meta[warp][stage][2 * mt + 1];
+        const float ks = meta[stream][stage][2 * mt], vs = meta[stream][stage][2 * mt + 1];
         // a block scaled by 0 holds zeros: its weight counts in l and its p V is 0 whatever p is
-        lv[mt] = vs > 0.f ? __log2f(vs) : 0.f;
-        iv[mt] = vs > 0.f ? __fdividef(1.f, vs) : 1.f;
-        if (!(vs == vs)) lv[mt] = vs;
+        dead[mi] = vs == 0.f;
+        const float lv = dead[mi] ? 0.f : __log2f(vs);
+        iv[mi] = dead[mi] ? 1.f : __fdividef(1.f, vs);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float v = fmaf(s[mt][t][i], f[t][i & 1] * ks, lv[mt]);
+            float v = fmaf(s[mi][t][i], f[t][i & 1] * ks, lv);
             if (edge && base + mt * 16 + j + (i >> 1) * 8 >= lim[t][i & 1]) v = -INFINITY;
-            s[mt][t][i] = v;
+            s[mi][t][i] = v;
           }
       }
-      float up[NT][2], mu[NT][2];
+      // ---- the running maximum
+      float top[NT][2];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float v = fmaxf(s[0][t][i], s[0][t][i + 2]);
+#pragma unroll
+          for (int mi = 1; mi < kMt; ++mi) v = fmaxf(v, fmaxf(s[mi][t][i], s[mi][t][i + 2]));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+          top[t][i] = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+        }
+      if (kPair) {
+        if (j == 0) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+            *reinterpret_cast<float2*>(&s_max[stream][sub][t * 8 + 2 * c]) = make_float2(top[t][0], top[t][1]);
+        }
+        pair_sync(stream);
+        // both warps are past the previous tile: its stage takes the tile kStages ahead
+        if (copies && alive && spent >= 0) {
+          put_scales();
+          copy(spent);
+          look_up();
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const float2 o = *reinterpret_cast<const float2*>(&s_max[stream][sub ^ 1][t * 8 + 2 * c]);
+          top[t][0] = fmaxf(top[t][0], o.x);
+          top[t][1] = fmaxf(top[t][1], o.y);
+        }
+      }
+      float mu[NT][2], up[NT][2];
       bool changed = false;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float v = fmaxf(fmaxf(s[0][t][i], s[0][t][i + 2]), fmaxf(s[1][t][i], s[1][t][i + 2]));
-          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
-          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
-          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-          const float now = fmaxf(m[t][i], v);
+          const float now = fmaxf(m[t][i], top[t][i]);
           mu[t][i] = (now == -INFINITY ? 0.f : now) - kShift;
           up[t][i] = fast_exp2(m[t][i] - kShift - mu[t][i]);
           changed |= now > m[t][i];
@@ -419,29 +496,42 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
 #pragma unroll
-          for (int k = 0; k < kChunks; ++k)
+          for (int k = 0; k < kOut; ++k)
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[k][t][i] *= up[t][i & 1];
           l[t][0] *= up[t][0];
           l[t][1] *= up[t][1];
         }
       }
-      // ---- p, its sum, and P^T as the B operand
+      // ---- p, its sum, and P^T as the B operand of the tile's two 16-token steps
       uint32_t pf[2][NT][2];
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        const float vs = meta[warp][stage][2 * mt + 1];
+      for (int mi = 0; mi < kMt; ++mi) {
+        const int at = kPair ? 0 : mi;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           float e[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            e[i] = fast_exp2(s[mt][t][i] - mu[t][i & 1]);
-            l[t][i & 1] = fmaf(e[i], iv[mt], l[t][i & 1]);
+            e[i] = fast_exp2(s[mi][t][i] - mu[t][i & 1]);
+            l[t][i & 1] = fmaf(e[i], iv[mi], l[t][i & 1]);
           }
-          if (vs == 0.f) e[0] = e[1] = e[2] = e[3] = 0.f;
-          pf[mt][t][0] = transpose8x8(pack_half(e[0], e[1]));
-          pf[mt][t][1] = transpose8x8(pack_half(e[2], e[3]));
+          if (dead[mi]) e[0] = e[1] = e[2] = e[3] = 0.f;
+          pf[at][t][0] = transpose8x8(pack_half(e[0], e[1]));
+          pf[at][t][1] = transpose8x8(pack_half(e[2], e[3]));
+        }
+      }
+      if (kPair) {   // pf[0]: this warp's tokens, pf[1]: the other's
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          s_p[stream][sub][2 * t][lane] = pf[0][t][0];
+          s_p[stream][sub][2 * t + 1][lane] = pf[0][t][1];
+        }
+        pair_sync(stream);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          pf[1][t][0] = s_p[stream][sub ^ 1][2 * t][lane];
+          pf[1][t][1] = s_p[stream][sub ^ 1][2 * t + 1][lane];
         }
       }
       // ---- O^T += V^T P^T. In a tile that ends inside the rows some query token sees, every query
@@ -449,20 +539,21 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
       // place holds (stale bytes behind the end, NaN in a later draft's row), p = 0 cannot cancel it.
       auto values = [&](int seen, bool all) {
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
+        for (int ti = 0; ti < 2; ++ti) {
+          const int mt = kPair ? sub ^ ti : ti;
           uint32_t b0[NT], b1[NT];
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             // column j of the operand is query row t * 8 + j: only this pass's rows
             const bool mine = all || (n - qn + (r0 + t * 8 + j) / G + 1) == seen;
-            b0[t] = mine ? pf[mt][t][0] : 0u;
-            b1[t] = mine ? pf[mt][t][1] : 0u;
+            b0[t] = mine ? pf[ti][t][0] : 0u;
+            b1[t] = mine ? pf[ti][t][1] : 0u;
           }
           const int tok = base + mt * 16 + 2 * c;
 #pragma unroll
-          for (int k = 0; k < kChunks; k += 2) {
+          for (int k = 0; k < kOut; k += 2) {
             uint32_t r[4];
-            ldmatrix4_trans(vbase + piece<D>(mt * 16 + (lane & 15), k + (lane >> 4)), r);
+            ldmatrix4_trans(vbase + piece<D>(mt * 16 + (lane & 15), out0 + k + (lane >> 4)), r);
             if (!all) {
               // a register holds two codes of token 2 c (low half) and two of token 2 c + 1
 #pragma unroll
@@ -492,16 +583,21 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
         }
       }
       // ---- the stage is free: scales and copy of the tile kStages ahead, look-up of the one after
-      __syncwarp();
-      put_scales();
-      copy(stage);
-      look_up();
+      // (pair mode: once the other warp is known to be done, at the next tile's first barrier)
+      spent = stage;
+      if (!kPair) {
+        __syncwarp();
+        if (alive) {
+          put_scales();
+          copy(stage);
+          look_up();
+        }
+      }
       if (++stage == kStages) {
         stage = 0;
         phase ^= 1;
       }
     }
-    // copies look up and write one tile late: the last scales of a finished range are never read
     // ---------------------------------------------------------------- the item's result
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -510,10 +606,27 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
         float v = l[t][i];
         v += __shfl_xor_sync(0xffffffffu, v, 4);
         v += __shfl_xor_sync(0xffffffffu, v, 8);
-        v += __shfl_xor_sync(0xffffffffu, v, 16);
-        l[t][i] = v;
+        l[t][i] = v + __shfl_xor_sync(0xffffffffu, v, 16);
       }
+    if (kPair) {   // each warp has the sums of its own tokens
+      pair_sync(stream);
+      if (j == 0) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+          *reinterpret_cast<float2*>(&s_max[stream][sub][t * 8 + 2 * c]) = make_float2(l[t][0], l[t][1]);
+      }
+      pair_sync(stream);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const float2 o0 = *reinterpret_cast<const float2*>(&s_max[stream][0][t * 8 + 2 * c]);
+        const float2 o1 = *reinterpret_cast<const float2*>(&s_max[stream][1][t * 8 + 2 * c]);
+        l[t][0] = o0.x + o1.x;
+        l[t][1] = o0.y + o1.y;
+      }
+      pair_sync(stream);
+    }
     const bool complete = p.tile == 0 && end == p.tiles;
+    const bool last = x >= x1;
     if (complete) {
 #pragma unroll
       for (int t = 0; t < NT; ++t)
@@ -522,19 +635,19 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
           const int r = t * 8 + 2 * c + i;
           if (r < rows) {
             const int qi = (r0 + r) / G, head = p.h * G + (r0 + r) % G;
-            const float inv = l[t][i] == 0.f ? 0.f : __frcp_rn(l[t][i]);
-            uint32_t* o = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.o) + ((long)(first + qi) * a.H + head) * D);
+            const float inv = row_inv(l[t][i]);
+            uint32_t* o = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.o) + ((long)(p.first + qi) * a.H + head) * D);
 #pragma unroll
-            for (int k = 0; k < kChunks; ++k) o[k * 8 + j] = pack16(a.q_dtype, acc[k][t][i] * inv, acc[k][t][i + 2] * inv);
-            if (j == 0 && a.lse != nullptr)
-              a.lse[(long)head * a.T + first + qi] = l[t][i] == 0.f ? -INFINITY : (m[t][i] - kShift + log2f(l[t][i])) * kLn2;
+            for (int k = 0; k < kOut; ++k)
+              o[(out0 + k) * 8 + j] = pack16(a.q_dtype, acc[k][t][i] * inv, acc[k][t][i + 2] * inv);
+            if (j == 0 && sub == 0 && a.lse != nullptr) a.lse[(long)head * a.T + p.first + qi] = row_lse(m[t][i], l[t][i]);
           }
         }
     } else {
-      // slot 0: the piece starts the worker's range; slot 1: it starts the item
-      const int slot = (x - (end - p.tile) == x0) ? 0 : 1;
-      float* po = L.o + ((size_t)worker * 2 + slot) * kRows * D;
-      float* pm = L.ml + ((size_t)worker * 2 + slot) * kRows * 2;
+      // the range's last piece stays in the stream's ring (free: all its tiles are consumed; the pair
+      // has just met), a first piece before another item goes to the workspace
+      const int slot = last ? 1 : 0;
+      float* po = last ? reinterpret_cast<float*>(ring) : ws.head + ((size_t)blockIdx.x * kStreams + stream) * kRows * D;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -543,76 +656,128 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
           if (r < rows) {
             float2* o = reinterpret_cast<float2*>(po + (size_t)r * D);
 #pragma unroll
-            for (int k = 0; k < kChunks; ++k) o[k * 8 + j] = make_float2(acc[k][t][i], acc[k][t][i + 2]);
-            if (j == 0) *reinterpret_cast<float2*>(pm + 2 * r) = make_float2(m[t][i], l[t][i]);
+            for (int k = 0; k < kOut; ++k) o[(out0 + k) * 8 + j] = make_float2(acc[k][t][i], acc[k][t][i + 2]);
+            if (j == 0 && sub == 0) {
+              s_ml[stream][slot][r][0] = m[t][i];
+              s_ml[stream][slot][r][1] = l[t][i];
+            }
           }
         }
+      if (lane == 0 && sub == 0) {
+        s_start[stream][slot] = x - (end - p.tile) - p.tile;
+        s_place[stream][slot] = p;
+      }
+    }
+  }
+  __syncthreads();
+
+  // ---------------------------------------------------------------- the CTA's pieces, item by item
+  // pieces in list order: stream by stream, slot 0 before slot 1; those of one item are neighbours
+  bool open = false;
+  for (int i = 0; i < 2 * kStreams;) {
+    const long long start = s_start[i >> 1][i & 1];
+    if (start < 0) {
+      ++i;
+      continue;
+    }
+    int e = i + 1;             // [i, e): this item's pieces (and empty slots)
+    while (e < 2 * kStreams && (s_start[e >> 1][e & 1] < 0 || s_start[e >> 1][e & 1] == start)) ++e;
+    const Place p = s_place[i >> 1][i & 1];
+    const int r0 = p.rt * kRows, rows = min(p.qn * G - r0, kRows);
+    const bool inside = start >= c0 && start + p.tiles <= c1;
+    const int piece_at = start < c0 ? 0 : 1;
+    if (!inside && piece_at == 1) {
+      open = true;
+      if (tid == 0) ws.straddle[blockIdx.x] = Straddle{p.b, p.h, p.rt, ctas.part_of(start + p.tiles - 1)};
+    }
+    for (int at = tid; at < rows * (D / 4); at += kWarps * 32) {
+      const int r = at / (D / 4), d = at % (D / 4);
+      float top = -INFINITY;
+      for (int k = i; k < e; ++k)
+        if (s_start[k >> 1][k & 1] >= 0) top = fmaxf(top, s_ml[k >> 1][k & 1][r][0]);
+      const float ref = top == -INFINITY ? 0.f : top;
+      float l = 0.f;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = i; k < e; ++k) {
+        if (s_start[k >> 1][k & 1] < 0) continue;
+        const float* src = (k & 1) ? reinterpret_cast<const float*>(ring_base + (k >> 1) * S::kRing)
+                                   : ws.head + ((size_t)blockIdx.x * kStreams + (k >> 1)) * kRows * D;
+        const float w = fast_exp2(s_ml[k >> 1][k & 1][r][0] - ref);
+        const float4 o = *reinterpret_cast<const float4*>(src + (size_t)r * D + 4 * d);
+        l = fmaf(w, s_ml[k >> 1][k & 1][r][1], l);
+        v.x = fmaf(w, o.x, v.x);
+        v.y = fmaf(w, o.y, v.y);
+        v.z = fmaf(w, o.z, v.z);
+        v.w = fmaf(w, o.w, v.w);
+      }
+      if (inside) {
+        const int qi = (r0 + r) / G, head = p.h * G + (r0 + r) % G;
+        const float inv = row_inv(l);
+        reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.o) + ((long)(p.first + qi) * a.H + head) * D)[d] =
+            make_uint2(pack16(a.q_dtype, v.x * inv, v.y * inv), pack16(a.q_dtype, v.z * inv, v.w * inv));
+        if (d == 0 && a.lse != nullptr) a.lse[(long)head * a.T + p.first + qi] = row_lse(top, l);
+      } else {
+        const size_t row = ((size_t)blockIdx.x * 2 + piece_at) * kRows + r;
+        reinterpret_cast<float4*>(ws.o + row * D)[d] = v;
+        if (d == 0) *reinterpret_cast<float2*>(ws.ml + row * 2) = make_float2(top, l);
+      }
+    }
+    i = e;
+  }
+  if (!open && tid == 0) ws.straddle[blockIdx.x] = Straddle{0, 0, 0, -1};
+
+  // ---------------------------------------------------------------- rows without an item
+  // (no cached rows, or query tokens that belong to no request): o = 0, lse = -inf
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+    int first;
+    const int qn = q_tokens(a, b, first);
+    const int t0 = b == 0 ? 0 : first, t1 = b + 1 < a.B ? (a.cu == nullptr ? b + 1 : min(max(a.cu[b + 1], 0), a.T)) : a.T;
+    for (int t = t0; t < t1; ++t) {
+      if (t >= first && t < first + qn && rows_of(a, b) > 0) continue;
+      uint32_t* o = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.o) + (long)t * a.H * D);
+      for (int i = tid; i < a.H * (D / 2); i += kWarps * 32) o[i] = 0u;
+      if (a.lse != nullptr)
+        for (int h = tid; h < a.H; h += kWarps * 32) a.lse[(long)h * a.T + t] = -INFINITY;
     }
   }
 }
 
-// One CTA per (query token, head): the pieces of its item in list order, (m, l, O) each.
-constexpr int kCombineWarps = 4;
+// One CTA per (CTA of the attention, row): where that CTA's last item goes on in the next ones, their
+// pieces of the row in list order.
+constexpr int kCombineWarps = 8;
 
 template <int D, int NT>
-__global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(AttnArgs a, int NW) {
+__global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(AttnArgs a) {
   constexpr int kRows = 8 * NT, kPer = D / 32;
   __shared__ float part[kCombineWarps][D];
   __shared__ float part_l[kCombineWarps];
   pdl_trigger();
   pdl_wait();
-  const int t = blockIdx.x / a.H, head = blockIdx.x % a.H;
+  const int cta = blockIdx.x, row = blockIdx.y, grid = gridDim.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Workspace ws = workspace_of(a.workspace, grid, Shape<D, NT>::kStreams, kRows, D);
+  const Straddle st = ws.straddle[cta];
+  if (st.last < 0) return;
   const int G = a.H / a.c.Hkv;
-  // the token's request
-  int b = t;
-  if (a.cu != nullptr) {
-    int lo = 0, hi = a.B;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (a.cu[mid] <= t) lo = mid;
-      else hi = mid;
-    }
-    b = lo;
-  }
   int first;
-  const int qn = q_tokens(a, b, first);
-  const int qi = t - first;
-  const Layout L = layout_of(a.workspace, a.B, NW, kRows);
-  const int n = rows_of(a, b);
-  const int tiles = (n + kTile - 1) / kTile;
-  uint16_t* out = reinterpret_cast<uint16_t*>(a.o) + ((long)t * a.H + head) * D;
-  if (qi < 0 || qi >= qn || tiles == 0) {   // no cached rows (or a token outside every request)
-    if (threadIdx.x < D / 2) reinterpret_cast<uint32_t*>(out)[threadIdx.x] = 0u;
-    if (threadIdx.x == 0 && a.lse != nullptr) a.lse[(long)head * a.T + t] = -INFINITY;
-    return;
-  }
-  const int rts = (qn * G + kRows - 1) / kRows;
-  const int r = qi * G + head % G, rt = r / kRows;
-  const long long W = L.prefix[a.B];
-  const long long start = L.prefix[b] + ((long long)(head / G) * rts + rt) * tiles, stop = start + tiles;
-  const int w0 = worker_of(start, W, NW), w1 = worker_of(stop - 1, W, NW);
-  if (w0 == w1) return;                     // finished by its only worker
-  const int row = r - rt * kRows;
-  // with fewer tiles than workers some ranges in between are empty
-  auto empty = [&](int w) { return W * w / NW == W * (w + 1) / NW; };
-  auto slot_of = [&](int w) { return (size_t)w * 2 + ((w == w0 && start > W * w / NW) ? 1 : 0); };
+  const int qn = q_tokens(a, st.b, first);
+  const int r = st.rt * kRows + row;
+  if (r >= qn * G) return;
+  const int last = st.last;
+  auto at = [&](int w) { return ((size_t)w * 2 + (w == cta ? 1 : 0)) * kRows + row; };
   float top = -INFINITY;
-  for (int w = w0 + lane; w <= w1; w += 32)
-    if (!empty(w)) top = fmaxf(top, L.ml[(slot_of(w) * kRows + row) * 2]);
+  for (int w = cta + lane; w <= last; w += 32) top = fmaxf(top, ws.ml[at(w) * 2]);
   top = warp_max(top);
-  const float base = top == -INFINITY ? 0.f : top;
+  const float ref = top == -INFINITY ? 0.f : top;
   float acc[kPer], l = 0.f;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
 #pragma unroll 4
-  for (int w = w0 + warp; w <= w1; w += kCombineWarps) {
-    if (empty(w)) continue;
-    const size_t at = slot_of(w) * kRows + row;
-    const float2 ml = *reinterpret_cast<const float2*>(L.ml + at * 2);
-    const float e = fast_exp2(ml.x - base);
+  for (int w = cta + warp; w <= last; w += kCombineWarps) {
+    const float2 ml = *reinterpret_cast<const float2*>(ws.ml + at(w) * 2);
+    const float e = fast_exp2(ml.x - ref);
     l = fmaf(e, ml.y, l);
-    const float* o = L.o + at * D + lane * kPer;
+    const float* o = ws.o + at(w) * D + lane * kPer;
 #pragma unroll
     for (int i = 0; i < kPer; i += 2) {
       const float2 v = *reinterpret_cast<const float2*>(o + i);
@@ -626,6 +791,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(AttnArgs a,
   __syncthreads();
   l = 0.f;
   for (int w = 0; w < kCombineWarps; ++w) l += part_l[w];
+  const int qi = r / G, head = st.h * G + r % G;
   if (threadIdx.x < D / 2) {
     float v0 = 0.f, v1 = 0.f;
 #pragma unroll
@@ -633,11 +799,11 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(AttnArgs a,
       v0 += part[w][2 * threadIdx.x];
       v1 += part[w][2 * threadIdx.x + 1];
     }
-    const float inv = l == 0.f ? 0.f : __frcp_rn(l);
-    reinterpret_cast<uint32_t*>(out)[threadIdx.x] = pack16(a.q_dtype, v0 * inv, v1 * inv);
+    const float inv = row_inv(l);
+    reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.o) + ((long)(first + qi) * a.H + head) * D)[threadIdx.x] =
+        pack16(a.q_dtype, v0 * inv, v1 * inv);
   }
-  if (threadIdx.x == 0 && a.lse != nullptr)
-    a.lse[(long)head * a.T + t] = l == 0.f ? -INFINITY : (top - kShift + log2f(l)) * kLn2;
+  if (threadIdx.x == 0 && a.lse != nullptr) a.lse[(long)head * a.T + first + qi] = row_lse(top, l);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -663,23 +829,25 @@ bool make_map(CUtensorMap* map, const uint8_t* base, const Cache& c) {
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Query rows of an item: 8 where a request's rows fit, else 16 (each tile's codes are converted
-// once for both column tiles).
-int column_tiles(const AttnArgs& a) { return a.max_q * (a.H / a.c.Hkv) <= 8 ? 1 : 2; }
+// Column tiles of 8 query rows an item has: the least that hold a request's rows, at most 5.
+int column_tiles(const AttnArgs& a) {
+  const long rows = (long)a.max_q * (a.H / a.c.Hkv);
+  return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 5;
+}
 
 template <int D, int NT, bool INT8>
 cudaError_t launch_attn(const AttnArgs& a, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
-  const int grid = a.num_sms;
-  const size_t smem = 1024 + size_t(kWarps) * Ring<D>::kStages * Ring<D>::kBytes + size_t(a.B + 1) * sizeof(long long);
+  using S = Shape<D, NT>;
+  const size_t ring = 1024 + size_t(S::kStreams) * S::kRing;
+  const size_t smem = ring + size_t(a.B + 1) * sizeof(long long);
   auto kernel = attn_kernel<D, NT, INT8>;
   cudaError_t e = once_per_device_kernel(reinterpret_cast<const void*>(kernel), [&] {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                int(1024 + size_t(kWarps) * Ring<D>::kStages * Ring<D>::kBytes + (kAttnMaxRows + 1) * sizeof(long long)));
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(ring + (kAttnMaxRows + 1) * sizeof(long long)));
   });
   if (e != cudaSuccess) return e;
-  e = launch_pdl(kernel, dim3(unsigned(grid)), dim3(kWarps * 32), smem, s, km, vm, a);
+  e = launch_pdl(kernel, dim3(unsigned(a.num_sms)), dim3(kWarps * 32), smem, s, km, vm, a);
   if (e != cudaSuccess) return e;
-  return launch_pdl(combine_kernel<D, NT>, dim3(unsigned(a.T) * unsigned(a.H)), dim3(kCombineWarps * 32), 0, s, a, grid * kWarps);
+  return launch_pdl(combine_kernel<D, NT>, dim3(unsigned(a.num_sms), S::kRows), dim3(kCombineWarps * 32), 0, s, a);
 }
 
 template <int D, int NT>
@@ -687,12 +855,21 @@ cudaError_t attn_code(const AttnArgs& a, const CUtensorMap& km, const CUtensorMa
   return a.c.code == kInt8 ? launch_attn<D, NT, true>(a, km, vm, s) : launch_attn<D, NT, false>(a, km, vm, s);
 }
 
+template <int D>
+cudaError_t attn_rows(const AttnArgs& a, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
+  switch (column_tiles(a)) {
+    case 1: return attn_code<D, 1>(a, km, vm, s);
+    case 2: return attn_code<D, 2>(a, km, vm, s);
+    case 3: return attn_code<D, 3>(a, km, vm, s);
+    default: return attn_code<D, 5>(a, km, vm, s);
+  }
+}
+
 }  // namespace
 
 size_t attention_workspace(const AttnArgs& a) {
-  const size_t workers = size_t(a.num_sms) * kWarps, rows = 8 * size_t(column_tiles(a));
-  return align256(size_t(a.B + 1) * sizeof(long long)) + align256(workers * 2 * rows * 2 * sizeof(float)) +
-         workers * 2 * rows * a.c.D * sizeof(float);
+  const int nt = column_tiles(a);
+  return workspace_of(nullptr, a.num_sms, nt > 2 ? kWarps / 2 : kWarps, 8 * nt, a.c.D).bytes;
 }
 
 const char* attention(const AttnArgs& a, cudaStream_t s) {
@@ -712,10 +889,7 @@ const char* attention(const AttnArgs& a, cudaStream_t s) {
   if (encode_fn() == nullptr) return "attention_kv8: cuTensorMapEncodeTiled is not available";
   CUtensorMap km, vm;
   if (!make_map(&km, c.k, c) || !make_map(&vm, c.v, c)) return "attention_kv8: the cache's strides do not make a tensor map";
-  const int nt = column_tiles(a);
-  cudaError_t e;
-  if (c.D == 64) e = nt == 1 ? attn_code<64, 1>(a, km, vm, s) : attn_code<64, 2>(a, km, vm, s);
-  else e = nt == 1 ? attn_code<128, 1>(a, km, vm, s) : attn_code<128, 2>(a, km, vm, s);
+  const cudaError_t e = c.D == 64 ? attn_rows<64>(a, km, vm, s) : attn_rows<128>(a, km, vm, s);
   return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
 }
 

@@ -39,19 +39,24 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kTile = 32;     // cached tokens a tile
 constexpr float kShift = 15.f;
+constexpr float kNone = -3e38f;   // the running maximum before any score (finite: differences stay numbers)
 constexpr float kLn2 = 0.6931471805599453f;
 
 // How the warps of a CTA share a tile stream. Up to 16 query rows (NT <= 2 column tiles): a stream a
-// warp. More (NT = 3 or 5): two warps a stream, which split the tile's tokens in the scores and the
-// head dims in O, so that up to 40 rows take one pass over the cache with their accumulators in
-// registers and no code is converted twice.
+// warp, a tile at a time. More (NT = 3 or 5): two warps a stream, two tiles at a time; each computes
+// the scores of one tile, they exchange the column maxima and P, and each accumulates half of O's
+// dims over both tiles. So up to 40 rows take one pass over the cache with their accumulators in
+// registers, and no code is converted twice.
 template <int D, int NT>
 struct Shape {
   static constexpr bool kPair = NT > 2;
   static constexpr int kRows = 8 * NT;                      // query rows of an item
   static constexpr int kStreams = kPair ? kWarps / 2 : kWarps;
   static constexpr int kBytes = 2 * kTile * D;              // K and V of a tile
-  static constexpr int kStages = 196608 / (kStreams * kBytes);   // 192 KB of rings: 3 to 12 stages
+  // pair: q's fragments are read from shared memory (80 registers a lane for 40 rows of 128 dims)
+  static constexpr int kQBytes = kPair ? kStreams * kRows * D * 2 : 0;
+  static constexpr int kStages = (196608 - kQBytes) / (kStreams * kBytes);   // 192 KB: 3 to 10 stages
+  static constexpr int kStep = kPair ? 2 : 1;               // tiles a step
   static constexpr int kRing = kStages * kBytes;
   static_assert(kRing >= kRows * D * 4, "a stream's last piece is left in its ring");
 };
@@ -177,27 +182,30 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
 attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, AttnArgs a) {
   using S = Shape<D, NT>;
   constexpr bool kPair = S::kPair;
-  constexpr int kStages = S::kStages, kBytes = S::kBytes, kRows = S::kRows, kStreams = S::kStreams;
+  constexpr int kStages = S::kStages, kBytes = S::kBytes, kRows = S::kRows, kStreams = S::kStreams, kStep = S::kStep;
   constexpr int kChunks = D / 16;                          // 16-dim pieces of a row
-  constexpr int kMt = kPair ? 1 : 2;                       // 16-token groups whose scores a warp computes
   constexpr int kOut = kPair ? kChunks / 2 : kChunks;      // pieces of O a warp accumulates
   extern __shared__ unsigned char raw[];
   unsigned char* ring_base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  long long* prefix = reinterpret_cast<long long*>(ring_base + kStreams * S::kRing);
+  uint2* q_frag = reinterpret_cast<uint2*>(ring_base + kStreams * S::kRing);   // pair: [stream][piece][tile][lane]
+  long long* prefix = reinterpret_cast<long long*>(ring_base + kStreams * S::kRing + S::kQBytes);
   __shared__ uint64_t bars[kStreams][kStages];
-  __shared__ float meta[kStreams][kStages][4];             // k scale and v scale of the tile's two halves
+  __shared__ float meta[kStreams][kStages][2][2];          // k scale and v scale of the tile's (two) pages
   __shared__ long long warp_tot[kWarps];
   __shared__ float s_ml[kStreams][2][kRows][2];            // (m, l) of the streams' pieces
   __shared__ long long s_start[kStreams][2];               // first tile of the piece's item; -1: no piece
   __shared__ Place s_place[kStreams][2];
   __shared__ float s_max[kPair ? kStreams : 1][2][kRows];  // pair: column maxima of the two warps
-  __shared__ uint32_t s_p[kPair ? kStreams : 1][2][kPair ? NT * 2 : 1][32];   // pair: their P^T fragments
+  __shared__ uint32_t s_p[kPair ? kStreams : 1][2][kPair ? NT * 4 : 1][32];   // pair: their P^T fragments
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int stream = kPair ? warp >> 1 : warp, sub = kPair ? warp & 1 : 0;
   const int G = a.H / a.c.Hkv, P = a.c.P, Hkv = a.c.Hkv;
+  // a tile lies in one page of 32 tokens or more, or in two of 16
+  const int halves = P == 16 ? 2 : 1;
   if (tid == 0) {
+    // a stage is full with its bytes (one arrival that announces them) and its pages' scales
     for (int w = 0; w < kStreams; ++w)
-      for (int i = 0; i < kStages; ++i) mbar_init(&bars[w][i], 1);
+      for (int i = 0; i < kStages; ++i) mbar_init(&bars[w][i], 1 + halves);
     fence_barrier_init();
     tma_prefetch_desc(&kmap);
     tma_prefetch_desc(&vmap);
@@ -262,87 +270,85 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
   };
 
   // ---------------------------------------------------------------- the copies' side (one warp a stream)
+  // One lane a page of up to kStep tiles (odd and even tiles of the range have lanes of their own); a
+  // page's id is looked up one turn ahead of its copies.
   unsigned char* ring = ring_base + stream * S::kRing;
-  // a tile lies in one page of 32 tokens or more, or in two of 16 (lane 1 brings the second half)
-  const int halves = P == 16 ? 2 : 1;
   const int box = min(P, kTile);
-  long long px = x0;          // next tile whose page is looked up
+  const int my_tile = lane / halves, my_half = lane % halves;   // of the step (lanes past them: none)
+  const bool copies = sub == 0;
+  long long px = x0 + my_tile;     // the lane's next tile
   Place pp{};
-  int next_page = -1, next_row = 0, next_h = 0;   // looked up, not yet copied
-  bool next_valid = false;
+  int next_page = -1, next_row = 0, next_h = 0;
+  bool next_tile = false, next_valid = false;   // there is a tile; it reaches into the lane's page
+  int put_stage = 0, put_tile = 0;              // the next copy's stage, and its tile modulo kStep
   auto look_up = [&] {
+    next_tile = my_tile < kStep && px < x1;
     next_valid = false;
-    if (px < x1) {
-      const int block = pp.tile * kTile / P + lane;
-      if (lane < halves && block * P < pp.n) {
-        next_page = a.table[(long)pp.b * a.width + block];
-        next_valid = true;
-      }
+    if (next_tile) {
+      const int block = pp.tile * kTile / P + my_half;
+      next_valid = block * P < pp.n;
+      if (next_valid) next_page = a.table[(long)pp.b * a.width + block];
       next_row = pp.tile * kTile % P;
       next_h = pp.h;
-      ++px;
-      if (++pp.tile == pp.tiles && px < x1) pp = place_of(px);
+      px += kStep;
+      pp.tile += kStep;
+      if (pp.tile >= pp.tiles && px < x1) pp = place_of(px);
     }
   };
-  float load_ks = 1.f, load_vs = 1.f;             // scales of the tile copied last
-  int load_stage = -1;
-  auto put_scales = [&] {
-    if (load_stage >= 0 && lane < halves) {
-      meta[stream][load_stage][2 * lane] = load_ks;
-      meta[stream][load_stage][2 * lane + 1] = load_vs;
-      if (halves == 1) {
-        meta[stream][load_stage][2] = load_ks;
-        meta[stream][load_stage][3] = load_vs;
-      }
-    }
-    load_stage = -1;
-  };
-  auto copy = [&](int stage) {
+  auto copy = [&](int tiles) {
+    const int ahead = my_tile >= put_tile ? my_tile - put_tile : my_tile - put_tile + kStep;
+    const bool turn = ahead < tiles;            // (lanes past kStep tiles have no tile)
+    int st = put_stage + ahead;
+    st = st >= kStages ? st - kStages : st;
     const uint32_t valid = __ballot_sync(0xffffffffu, next_valid);
-    if (valid == 0) return;
-    uint64_t* bar = &bars[stream][stage];
-    if (lane == 0) mbar_arrive_expect_tx(bar, uint32_t(__popc(valid)) * 2u * uint32_t(box) * D);
-    __syncwarp();
-    load_ks = load_vs = 1.f;
-    if (next_valid) {
-      unsigned char* dst = ring + stage * kBytes + lane * 16 * D;
-      // a page id outside the pool reads as zeros (the tensor map's bounds)
-      tma_load_4d(dst, &kmap, bar, next_row, next_h, next_page);
-      tma_load_4d(dst + kTile * D, &vmap, bar, next_row, next_h, next_page);
-      if (next_page >= 0 && next_page < a.c.pages) {
+    if (turn && next_tile) {
+      uint64_t* bar = &bars[stream][st];
+      if (my_half == 0) {
+        const uint32_t mine = (valid >> lane) & (halves == 2 ? 3u : 1u);
+        mbar_arrive_expect_tx(bar, uint32_t(__popc(mine)) * 2u * uint32_t(box) * D);
+      }
+      float* sc = meta[stream][st][my_half];
+      if (next_valid) {
+        unsigned char* dst = ring + st * kBytes + my_half * 16 * D;
+        // a page id outside the pool reads as zeros (the tensor map's bounds)
+        tma_load_4d(dst, &kmap, bar, next_row, next_h, next_page);
+        tma_load_4d(dst + kTile * D, &vmap, bar, next_row, next_h, next_page);
+      }
+      if (next_valid && next_page >= 0 && next_page < a.c.pages) {
         const long at = (long)next_page * a.c.scale_page_stride + (long)next_h * a.c.scale_head_stride;
-        load_ks = a.c.k_scale[at];
-        load_vs = a.c.v_scale[at];
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(sc)), "l"(a.c.k_scale + at) : "memory");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(sc + 1)), "l"(a.c.v_scale + at) : "memory");
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
       } else {
-        report_error(a.status, int(StatusCode::kOutOfBounds), 411, next_page, next_h);
+        if (next_valid) report_error(a.status, int(StatusCode::kOutOfBounds), 411, next_page, next_h);
+        sc[0] = sc[1] = 1.f;
+        mbar_arrive(bar);
       }
     }
-    load_stage = stage;
+    if (turn) look_up();
+    put_stage += tiles;
+    put_stage = put_stage >= kStages ? put_stage - kStages : put_stage;
+    put_tile = (put_tile + tiles) % kStep;
   };
-  const bool copies = sub == 0;
   if (copies && x0 < x1) {
-    pp = place_of(px);
+    if (px < x1) pp = place_of(px);
     look_up();
 #pragma unroll 1
-    for (int i = 0; i < kStages; ++i) {
-      put_scales();
-      copy(i);
-      look_up();
-    }
-    put_scales();
+    for (int i = 0; i < kStages; i += kStep) copy(min(kStep, kStages - i));
   }
-  if (kPair) pair_sync(stream);
-  else __syncwarp();
+  __syncwarp();
 
   // ---------------------------------------------------------------- the products' side
   const int j = lane >> 2, c = lane & 3;   // fragment row and column group of the lane
   const int out0 = sub * kOut;             // first piece of O of this warp
-  int stage = 0, spent = -1;               // spent: pair mode, the stage both warps are done with
-  uint32_t phase = 0;
+  int stage = 0;
+  uint32_t phase = 0;                      // of `stage`; a stage before it in the ring is one phase on
+  int spent = 0;                           // pair mode: stages that take copies at the next step
   long long x = x0;
   // A wait that ran out (reported) ends the waiting and the copies, not the loop: the barriers that two
   // warps share stay matched, and the rest of the range is computed on whatever the ring holds.
   bool alive = true;
+  auto stage_at = [&](int i) { return stage + i >= kStages ? stage + i - kStages : stage + i; };
   while (x < x1) {
     const Place p = place_of(x);
     const int n = p.n, qn = p.qn;
@@ -351,7 +357,8 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
 
     // q as the f16 B operand: lane (j, c) holds row j of each column tile, dims 16 s + 4 c .. + 3 of
     // k step s (the same order in which a lane's K bytes come out of ldmatrix)
-    uint32_t qf[NT][kChunks][2];
+    uint32_t qf[kPair ? 1 : NT][kPair ? 1 : kChunks][2];
+    uint2* qs = q_frag + stream * kChunks * NT * 32 + lane;
     float f[NT][2];          // score factor of the lane's two columns
     int lim[NT][2];          // rows seen by them
     float m[NT][2], l[NT][2];
@@ -384,8 +391,13 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
       const float up = pow2(e);
 #pragma unroll
       for (int s = 0; s < kChunks; ++s) {
-        qf[t][s][0] = pack_half(v[s][0] * up, v[s][1] * up);
-        qf[t][s][1] = pack_half(v[s][2] * up, v[s][3] * up);
+        const uint32_t lo = pack_half(v[s][0] * up, v[s][1] * up), hi = pack_half(v[s][2] * up, v[s][3] * up);
+        if constexpr (kPair) {
+          if (sub == (t & 1)) qs[(s * NT + t) * 32] = make_uint2(lo, hi);
+        } else {
+          qf[t][s][0] = lo;
+          qf[t][s][1] = hi;
+        }
       }
       const float back = a.scale * 1.4426950408889634f * pow2(-e);
 #pragma unroll
@@ -393,7 +405,7 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
         f[t][i] = __shfl_sync(0xffffffffu, back, (2 * c + i) * 4);
         const int col = t * 8 + 2 * c + i;
         lim[t][i] = col < rows ? n - qn + (r0 + col) / G + 1 : n;
-        m[t][i] = -INFINITY;
+        m[t][i] = kNone;
         l[t][i] = 0.f;
       }
 #pragma unroll
@@ -401,27 +413,43 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[s][t][i] = 0.f;
     }
+    if (kPair) pair_sync(stream);
     const int qi0 = r0 / G, qi1 = (r0 + rows - 1) / G;    // the item's query tokens
     const int least = n - qn + qi0 + 1;                   // rows that all of them see
 
-    for (int tile = p.tile; tile < end; ++tile, ++x) {
-      if (alive) alive = mbar_wait(&bars[stream][stage], phase, a.status, 412);
-      const int base = tile * kTile;
-      const uint32_t kbase = smem_u32(ring + stage * kBytes), vbase = kbase + kTile * D;
-      const bool edge = base + kTile > least;
-      // ---- S^T = K Q^T, in the log2 domain, masked
-      float s[kMt][NT][4];
-      float iv[kMt];
-      bool dead[kMt];
+    for (int tile = p.tile; tile < end; tile += kStep) {
+      const int count = min(kStep, end - tile);           // tiles of this step
 #pragma unroll
-      for (int mi = 0; mi < kMt; ++mi) {
-        const int mt = kPair ? sub : mi;
+      for (int q = 0; q < kStep; ++q)
+        if (alive && q < count) alive = mbar_wait(&bars[stream][stage_at(q)], stage + q >= kStages ? phase ^ 1 : phase, a.status, 412);
+      const int base = tile * kTile;
+      const uint32_t ring_at = smem_u32(ring);
+      const bool edge = base + kStep * kTile > least || count < kStep;
+      const bool idle = sub >= count;                     // no tile for this warp in this step
+      const int k_stage = stage_at(sub);
+      const uint32_t kbase = ring_at + k_stage * kBytes;
+      // ---- S^T = K Q^T of this warp's tile
+      float s[2][NT][4];
+      float iv[2];
+      bool dead[2];
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[mi][t][i] = 0.f;
+          for (int i = 0; i < 4; ++i) s[mt][t][i] = 0.f;
 #pragma unroll
-        for (int k = 0; k < kChunks; k += 2) {
+      for (int k = 0; k < kChunks; k += 2) {
+        uint2 qb[2][NT];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            if constexpr (kPair) qb[h][t] = qs[((k + h) * NT + t) * 32];
+            else qb[h][t] = make_uint2(qf[t][k + h][0], qf[t][k + h][1]);
+          }
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
           uint32_t r[4];
           ldmatrix4(kbase + piece<D>(mt * 16 + (lane & 15), k + (lane >> 4)), r);
 #pragma unroll
@@ -430,32 +458,41 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
             decode4<INT8>(r[2 * h], af[0], af[2]);
             decode4<INT8>(r[2 * h + 1], af[1], af[3]);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) mma_f16(s[mi][t], af, qf[t][k + h][0], qf[t][k + h][1]);
+            for (int t = 0; t < NT; ++t) mma_f16(s[mt][t], af, qb[h][t].x, qb[h][t].y);
           }
         }
-        const float ks = meta[stream][stage][2 * mt], vs = meta[stream][stage][2 * mt + 1];
-        // a block scaled by 0 holds zeros: its weight counts in l and its p V is 0 whatever p is
-        dead[mi] = vs == 0.f;
-        const float lv = dead[mi] ? 0.f : __log2f(vs);
-        iv[mi] = dead[mi] ? 1.f : __fdividef(1.f, vs);
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float v = fmaf(s[mi][t][i], f[t][i & 1] * ks, lv);
-            if (edge && base + mt * 16 + j + (i >> 1) * 8 >= lim[t][i & 1]) v = -INFINITY;
-            s[mi][t][i] = v;
-          }
       }
-      // ---- the running maximum
+      // ---- in the log2 domain, masked; the running maximum
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        const int half = halves == 2 ? mt : 0;
+        const float ks = meta[stream][k_stage][half][0], vs = meta[stream][k_stage][half][1];
+        // a block scaled by 0 holds zeros: its weight counts in l and its p V is 0 whatever p is
+        dead[mt] = vs == 0.f || idle;
+        const float lv = dead[mt] ? 0.f : __log2f(vs);
+        iv[mt] = dead[mt] ? 1.f : __fdividef(1.f, vs);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const float f0 = f[t][0] * ks, f1 = f[t][1] * ks;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[mt][t][i] = fmaf(s[mt][t][i], i & 1 ? f1 : f0, lv);
+        }
+      }
+      if (edge) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (idle || base + sub * kTile + mt * 16 + j + (i >> 1) * 8 >= lim[t][i & 1]) s[mt][t][i] = -INFINITY;
+      }
       float top[NT][2];
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float v = fmaxf(s[0][t][i], s[0][t][i + 2]);
-#pragma unroll
-          for (int mi = 1; mi < kMt; ++mi) v = fmaxf(v, fmaxf(s[mi][t][i], s[mi][t][i + 2]));
+          float v = fmaxf(fmaxf(s[0][t][i], s[0][t][i + 2]), fmaxf(s[1][t][i], s[1][t][i + 2]));
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
           top[t][i] = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
@@ -467,12 +504,8 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
             *reinterpret_cast<float2*>(&s_max[stream][sub][t * 8 + 2 * c]) = make_float2(top[t][0], top[t][1]);
         }
         pair_sync(stream);
-        // both warps are past the previous tile: its stage takes the tile kStages ahead
-        if (copies && alive && spent >= 0) {
-          put_scales();
-          copy(spent);
-          look_up();
-        }
+        // both warps are past the previous step: its stages take the next copies
+        if (copies && alive && spent > 0) copy(spent);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           const float2 o = *reinterpret_cast<const float2*>(&s_max[stream][sub ^ 1][t * 8 + 2 * c]);
@@ -480,76 +513,74 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
           top[t][1] = fmaxf(top[t][1], o.y);
         }
       }
-      float mu[NT][2], up[NT][2];
       bool changed = false;
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float now = fmaxf(m[t][i], top[t][i]);
-          mu[t][i] = (now == -INFINITY ? 0.f : now) - kShift;
-          up[t][i] = fast_exp2(m[t][i] - kShift - mu[t][i]);
-          changed |= now > m[t][i];
-          m[t][i] = now;
-        }
+      for (int t = 0; t < NT; ++t) changed |= top[t][0] > m[t][0] || top[t][1] > m[t][1];
       if (__any_sync(0xffffffffu, changed)) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
+          float up[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float now = fmaxf(m[t][i], top[t][i]);
+            up[i] = fast_exp2(m[t][i] - now);
+            m[t][i] = now;
+            l[t][i] *= up[i];
+          }
 #pragma unroll
           for (int k = 0; k < kOut; ++k)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[k][t][i] *= up[t][i & 1];
-          l[t][0] *= up[t][0];
-          l[t][1] *= up[t][1];
+            for (int i = 0; i < 4; ++i) acc[k][t][i] *= up[i & 1];
         }
       }
       // ---- p, its sum, and P^T as the B operand of the tile's two 16-token steps
       uint32_t pf[2][NT][2];
 #pragma unroll
-      for (int mi = 0; mi < kMt; ++mi) {
-        const int at = kPair ? 0 : mi;
+      for (int t = 0; t < NT; ++t) {
+        const float mu[2] = {m[t][0] - kShift, m[t][1] - kShift};
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
+        for (int mt = 0; mt < 2; ++mt) {
           float e[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            e[i] = fast_exp2(s[mi][t][i] - mu[t][i & 1]);
-            l[t][i & 1] = fmaf(e[i], iv[mi], l[t][i & 1]);
+            e[i] = fast_exp2(s[mt][t][i] - mu[i & 1]);
+            l[t][i & 1] = fmaf(e[i], iv[mt], l[t][i & 1]);
           }
-          if (dead[mi]) e[0] = e[1] = e[2] = e[3] = 0.f;
-          pf[at][t][0] = transpose8x8(pack_half(e[0], e[1]));
-          pf[at][t][1] = transpose8x8(pack_half(e[2], e[3]));
+          const uint32_t lo = pack_half(e[0], e[1]), hi = pack_half(e[2], e[3]);
+          pf[mt][t][0] = transpose8x8(dead[mt] ? 0u : lo);
+          pf[mt][t][1] = transpose8x8(dead[mt] ? 0u : hi);
         }
       }
-      if (kPair) {   // pf[0]: this warp's tokens, pf[1]: the other's
+      if (kPair) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          s_p[stream][sub][2 * t][lane] = pf[0][t][0];
-          s_p[stream][sub][2 * t + 1][lane] = pf[0][t][1];
-        }
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) s_p[stream][sub][(mt * NT + t) * 2 + i][lane] = pf[mt][t][i];
         pair_sync(stream);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          pf[1][t][0] = s_p[stream][sub ^ 1][2 * t][lane];
-          pf[1][t][1] = s_p[stream][sub ^ 1][2 * t + 1][lane];
-        }
       }
-      // ---- O^T += V^T P^T. In a tile that ends inside the rows some query token sees, every query
+      // ---- O^T += V^T P^T. In a step that ends inside the rows some query token sees, every query
       // token gets a pass of its own with the codes it must not see taken as 0: whatever a masked
       // place holds (stale bytes behind the end, NaN in a later draft's row), p = 0 cannot cancel it.
-      auto values = [&](int seen, bool all) {
+      auto values = [&](int q, int seen, bool all) {
+        const uint32_t vbase = ring_at + stage_at(q) * kBytes + kTile * D;
 #pragma unroll
-        for (int ti = 0; ti < 2; ++ti) {
-          const int mt = kPair ? sub ^ ti : ti;
+        for (int mt = 0; mt < 2; ++mt) {
           uint32_t b0[NT], b1[NT];
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
+            if constexpr (kPair) {
+              b0[t] = s_p[stream][q][(mt * NT + t) * 2][lane];
+              b1[t] = s_p[stream][q][(mt * NT + t) * 2 + 1][lane];
+            } else {
+              b0[t] = pf[mt][t][0];
+              b1[t] = pf[mt][t][1];
+            }
             // column j of the operand is query row t * 8 + j: only this pass's rows
-            const bool mine = all || (n - qn + (r0 + t * 8 + j) / G + 1) == seen;
-            b0[t] = mine ? pf[ti][t][0] : 0u;
-            b1[t] = mine ? pf[ti][t][1] : 0u;
+            if (!all && (n - qn + (r0 + t * 8 + j) / G + 1) != seen) b0[t] = b1[t] = 0u;
           }
-          const int tok = base + mt * 16 + 2 * c;
+          const int tok = base + q * kTile + mt * 16 + 2 * c;
 #pragma unroll
           for (int k = 0; k < kOut; k += 2) {
             uint32_t r[4];
@@ -574,27 +605,28 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
         }
       };
       if (!edge) {
-        values(0, true);
+#pragma unroll
+        for (int q = 0; q < kStep; ++q) values(q, 0, true);
       } else {
 #pragma unroll 1
         for (int qi = qi0; qi <= qi1; ++qi) {
           const int seen = n - qn + qi + 1;
-          if (seen > base) values(seen, false);
+#pragma unroll 1
+          for (int q = 0; q < count; ++q)
+            if (seen > base + q * kTile) values(q, seen, false);
         }
       }
-      // ---- the stage is free: scales and copy of the tile kStages ahead, look-up of the one after
-      // (pair mode: once the other warp is known to be done, at the next tile's first barrier)
-      spent = stage;
+      // ---- the stages are free (pair mode: once the other warp is known to be done with them, at the
+      // next step's first barrier)
+      spent = count;
+      x += count;
       if (!kPair) {
         __syncwarp();
-        if (alive) {
-          put_scales();
-          copy(stage);
-          look_up();
-        }
+        if (alive) copy(1);
       }
-      if (++stage == kStages) {
-        stage = 0;
+      stage += count;
+      if (stage >= kStages) {
+        stage -= kStages;
         phase ^= 1;
       }
     }
@@ -692,17 +724,16 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
     }
     for (int at = tid; at < rows * (D / 4); at += kWarps * 32) {
       const int r = at / (D / 4), d = at % (D / 4);
-      float top = -INFINITY;
+      float top = kNone;
       for (int k = i; k < e; ++k)
         if (s_start[k >> 1][k & 1] >= 0) top = fmaxf(top, s_ml[k >> 1][k & 1][r][0]);
-      const float ref = top == -INFINITY ? 0.f : top;
       float l = 0.f;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int k = i; k < e; ++k) {
         if (s_start[k >> 1][k & 1] < 0) continue;
         const float* src = (k & 1) ? reinterpret_cast<const float*>(ring_base + (k >> 1) * S::kRing)
                                    : ws.head + ((size_t)blockIdx.x * kStreams + (k >> 1)) * kRows * D;
-        const float w = fast_exp2(s_ml[k >> 1][k & 1][r][0] - ref);
+        const float w = fast_exp2(s_ml[k >> 1][k & 1][r][0] - top);
         const float4 o = *reinterpret_cast<const float4*>(src + (size_t)r * D + 4 * d);
         l = fmaf(w, s_ml[k >> 1][k & 1][r][1], l);
         v.x = fmaf(w, o.x, v.x);
@@ -765,17 +796,16 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(AttnArgs a)
   if (r >= qn * G) return;
   const int last = st.last;
   auto at = [&](int w) { return ((size_t)w * 2 + (w == cta ? 1 : 0)) * kRows + row; };
-  float top = -INFINITY;
+  float top = kNone;
   for (int w = cta + lane; w <= last; w += 32) top = fmaxf(top, ws.ml[at(w) * 2]);
   top = warp_max(top);
-  const float ref = top == -INFINITY ? 0.f : top;
   float acc[kPer], l = 0.f;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
 #pragma unroll 4
   for (int w = cta + warp; w <= last; w += kCombineWarps) {
     const float2 ml = *reinterpret_cast<const float2*>(ws.ml + at(w) * 2);
-    const float e = fast_exp2(ml.x - ref);
+    const float e = fast_exp2(ml.x - top);
     l = fmaf(e, ml.y, l);
     const float* o = ws.o + at(w) * D + lane * kPer;
 #pragma unroll
@@ -838,7 +868,7 @@ int column_tiles(const AttnArgs& a) {
 template <int D, int NT, bool INT8>
 cudaError_t launch_attn(const AttnArgs& a, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
   using S = Shape<D, NT>;
-  const size_t ring = 1024 + size_t(S::kStreams) * S::kRing;
+  const size_t ring = 1024 + size_t(S::kStreams) * S::kRing + S::kQBytes;
   const size_t smem = ring + size_t(a.B + 1) * sizeof(long long);
   auto kernel = attn_kernel<D, NT, INT8>;
   cudaError_t e = once_per_device_kernel(reinterpret_cast<const void*>(kernel), [&] {

@@ -26,6 +26,8 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <algorithm>
+
 #include "kv8_common.cuh"
 #include "launch.h"
 
@@ -62,9 +64,12 @@ struct Shape {
 };
 
 // An item (request, KV head, query row tile) that goes on in the next CTA.
-struct Straddle {
-  int b, h, rt;
+struct __align__(16) Straddle {
   int last;            // the last CTA that works on it; -1: none
+  int row0, rows;      // its query rows (token * G + head of the group, within the request)
+  int first;           // the request's first query token
+  int head;            // first query head of the KV head
+  int pad[3];
 };
 
 struct Workspace {
@@ -92,14 +97,19 @@ __host__ __device__ inline Workspace workspace_of(void* ws, int ctas, int stream
   return w;
 }
 
+// 64-bit quotient, by 32-bit division where both fit.
+__device__ __forceinline__ long long quotient(long long x, long long y) {
+  return ((x | y) >> 32) == 0 ? (long long)(uint32_t(x) / uint32_t(y)) : x / y;
+}
+
 // The tile list in `n` equal ranges: part i starts at begin(i).
 struct Split {
   long long q, r;
-  __device__ __forceinline__ Split(long long total, int n) : q(total / n), r(total % n) {}
+  __device__ __forceinline__ Split(long long total, int n) : q(quotient(total, n)), r(total - q * n) {}
   __device__ __forceinline__ long long begin(int i) const { return q * i + min((long long)i, r); }
   __device__ __forceinline__ int part_of(long long x) const {   // the part that holds x
     const long long big = r * (q + 1);
-    return int(x < big ? x / (q + 1) : r + (x - big) / q);
+    return int(x < big ? quotient(x, q + 1) : r + quotient(x - big, q));
   }
 };
 
@@ -189,6 +199,8 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
   unsigned char* ring_base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint2* q_frag = reinterpret_cast<uint2*>(ring_base + kStreams * S::kRing);   // pair: [stream][piece][tile][lane]
   long long* prefix = reinterpret_cast<long long*>(ring_base + kStreams * S::kRing + S::kQBytes);
+  int* s_rows = reinterpret_cast<int*>(prefix + a.B + 1);    // cached rows of each request
+  int* s_first = s_rows + a.B;                               // its first query token, and (next B) their number
   __shared__ uint64_t bars[kStreams][kStages];
   __shared__ float meta[kStreams][kStages][2][2];          // k scale and v scale of the tile's (two) pages
   __shared__ long long warp_tot[kWarps];
@@ -219,12 +231,16 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
     const int per = (a.B + kWarps * 32 - 1) / (kWarps * 32);
     const int r0 = min(a.B, tid * per), r1 = min(a.B, r0 + per);
     auto tiles_of = [&](int b) {
-      int first;
-      const int qn = q_tokens(a, b, first);
-      return (long long)Hkv * ((qn * G + kRows - 1) / kRows) * ((rows_of(a, b) + kTile - 1) / kTile);
+      return (long long)Hkv * ((s_first[a.B + b] * G + kRows - 1) / kRows) * ((s_rows[b] + kTile - 1) / kTile);
     };
     long long own = 0;
-    for (int b = r0; b < r1; ++b) own += tiles_of(b);
+    for (int b = r0; b < r1; ++b) {
+      int first;
+      s_first[a.B + b] = q_tokens(a, b, first);
+      s_first[b] = first;
+      s_rows[b] = rows_of(a, b);
+      own += tiles_of(b);
+    }
     long long inc = own;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -257,12 +273,13 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
     }
     Place p;
     p.b = lo;
-    p.qn = q_tokens(a, lo, p.first);
-    p.n = rows_of(a, lo);
+    p.first = s_first[lo];
+    p.qn = s_first[a.B + lo];
+    p.n = s_rows[lo];
     const int rts = (p.qn * G + kRows - 1) / kRows;
     p.tiles = (p.n + kTile - 1) / kTile;
     const long long rem = x - prefix[lo];
-    const int item = int(rem / p.tiles);
+    const int item = int(quotient(rem, p.tiles));
     p.tile = int(rem - (long long)item * p.tiles);
     p.h = item / rts;
     p.rt = item - p.h * rts;
@@ -337,6 +354,24 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
     for (int i = 0; i < kStages; i += kStep) copy(min(kStep, kStages - i));
   }
   __syncwarp();
+
+  // ---------------------------------------------------------------- rows without an item
+  // (no cached rows, or query tokens that belong to no request): o = 0, lse = -inf
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+    const int first = s_first[b], qn = s_first[a.B + b];
+    const bool some = s_rows[b] > 0;
+    const int t0 = b == 0 ? 0 : first, t1 = b + 1 < a.B ? s_first[b + 1] : a.T;
+    for (int t = t0; t < min(t1, a.T); ++t) {
+      if (some && t >= first) {           // tokens first .. first + qn - 1 have one
+        t = max(t, first + qn - 1);
+        if (t >= first && t < first + qn) continue;
+      }
+      uint32_t* o = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.o) + (long)t * a.H * D);
+      for (int i = tid; i < a.H * (D / 2); i += kWarps * 32) o[i] = 0u;
+      if (a.lse != nullptr)
+        for (int h = tid; h < a.H; h += kWarps * 32) a.lse[(long)h * a.T + t] = -INFINITY;
+    }
+  }
 
   // ---------------------------------------------------------------- the products' side
   const int j = lane >> 2, c = lane & 3;   // fragment row and column group of the lane
@@ -704,136 +739,124 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
   __syncthreads();
 
   // ---------------------------------------------------------------- the CTA's pieces, item by item
-  // pieces in list order: stream by stream, slot 0 before slot 1; those of one item are neighbours
+  // bit 2 i + k of a mask: piece k of stream i. Every warp finds the items by itself.
+  const long long my_start = lane < 2 * kStreams ? s_start[lane >> 1][lane & 1] : -1;
+  const uint32_t same = __match_any_sync(0xffffffffu, my_start);
+  uint32_t leaders = __ballot_sync(0xffffffffu, my_start >= 0 && __ffs(same) - 1 == lane);
   bool open = false;
-  for (int i = 0; i < 2 * kStreams;) {
-    const long long start = s_start[i >> 1][i & 1];
-    if (start < 0) {
-      ++i;
-      continue;
-    }
-    int e = i + 1;             // [i, e): this item's pieces (and empty slots)
-    while (e < 2 * kStreams && (s_start[e >> 1][e & 1] < 0 || s_start[e >> 1][e & 1] == start)) ++e;
-    const Place p = s_place[i >> 1][i & 1];
+  while (leaders) {
+    const int lead = __ffs(leaders) - 1;
+    leaders &= leaders - 1;
+    const uint32_t mask = __shfl_sync(0xffffffffu, same, lead);
+    const long long start = __shfl_sync(0xffffffffu, my_start, lead);
+    const Place& p = s_place[lead >> 1][lead & 1];
+    const int tiles = p.tiles, h = p.h, first = p.first;
     const int r0 = p.rt * kRows, rows = min(p.qn * G - r0, kRows);
-    const bool inside = start >= c0 && start + p.tiles <= c1;
+    const bool inside = start >= c0 && start + tiles <= c1;
     const int piece_at = start < c0 ? 0 : 1;
     if (!inside && piece_at == 1) {
       open = true;
-      if (tid == 0) ws.straddle[blockIdx.x] = Straddle{p.b, p.h, p.rt, ctas.part_of(start + p.tiles - 1)};
+      if (tid == 0) ws.straddle[blockIdx.x] = Straddle{ctas.part_of(start + tiles - 1), r0, rows, first, h * G, {0, 0, 0}};
     }
     for (int at = tid; at < rows * (D / 4); at += kWarps * 32) {
       const int r = at / (D / 4), d = at % (D / 4);
       float top = kNone;
-      for (int k = i; k < e; ++k)
-        if (s_start[k >> 1][k & 1] >= 0) top = fmaxf(top, s_ml[k >> 1][k & 1][r][0]);
+#pragma unroll
+      for (int k = 0; k < 2 * kStreams; ++k)
+        if (mask >> k & 1) top = fmaxf(top, s_ml[k >> 1][k & 1][r][0]);
       float l = 0.f;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int k = i; k < e; ++k) {
-        if (s_start[k >> 1][k & 1] < 0) continue;
-        const float* src = (k & 1) ? reinterpret_cast<const float*>(ring_base + (k >> 1) * S::kRing)
-                                   : ws.head + ((size_t)blockIdx.x * kStreams + (k >> 1)) * kRows * D;
+      auto add = [&](int k, const float4 o) {
         const float w = fast_exp2(s_ml[k >> 1][k & 1][r][0] - top);
-        const float4 o = *reinterpret_cast<const float4*>(src + (size_t)r * D + 4 * d);
         l = fmaf(w, s_ml[k >> 1][k & 1][r][1], l);
         v.x = fmaf(w, o.x, v.x);
         v.y = fmaf(w, o.y, v.y);
         v.z = fmaf(w, o.z, v.z);
         v.w = fmaf(w, o.w, v.w);
-      }
+      };
+#pragma unroll
+      for (int k = 0; k < 2 * kStreams; ++k)
+        if (mask >> k & 1)
+          add(k, (k & 1) ? *reinterpret_cast<const float4*>(ring_base + (k >> 1) * S::kRing + ((size_t)r * D + 4 * d) * 4)
+                         : *reinterpret_cast<const float4*>(ws.head + (((size_t)blockIdx.x * kStreams + (k >> 1)) * kRows + r) * D + 4 * d));
       if (inside) {
-        const int qi = (r0 + r) / G, head = p.h * G + (r0 + r) % G;
+        const int qi = (r0 + r) / G, head = h * G + (r0 + r) % G;
         const float inv = row_inv(l);
-        reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.o) + ((long)(p.first + qi) * a.H + head) * D)[d] =
+        reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.o) + ((long)(first + qi) * a.H + head) * D)[d] =
             make_uint2(pack16(a.q_dtype, v.x * inv, v.y * inv), pack16(a.q_dtype, v.z * inv, v.w * inv));
-        if (d == 0 && a.lse != nullptr) a.lse[(long)head * a.T + p.first + qi] = row_lse(top, l);
+        if (d == 0 && a.lse != nullptr) a.lse[(long)head * a.T + first + qi] = row_lse(top, l);
       } else {
         const size_t row = ((size_t)blockIdx.x * 2 + piece_at) * kRows + r;
         reinterpret_cast<float4*>(ws.o + row * D)[d] = v;
         if (d == 0) *reinterpret_cast<float2*>(ws.ml + row * 2) = make_float2(top, l);
       }
     }
-    i = e;
   }
-  if (!open && tid == 0) ws.straddle[blockIdx.x] = Straddle{0, 0, 0, -1};
-
-  // ---------------------------------------------------------------- rows without an item
-  // (no cached rows, or query tokens that belong to no request): o = 0, lse = -inf
-  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
-    int first;
-    const int qn = q_tokens(a, b, first);
-    const int t0 = b == 0 ? 0 : first, t1 = b + 1 < a.B ? (a.cu == nullptr ? b + 1 : min(max(a.cu[b + 1], 0), a.T)) : a.T;
-    for (int t = t0; t < t1; ++t) {
-      if (t >= first && t < first + qn && rows_of(a, b) > 0) continue;
-      uint32_t* o = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.o) + (long)t * a.H * D);
-      for (int i = tid; i < a.H * (D / 2); i += kWarps * 32) o[i] = 0u;
-      if (a.lse != nullptr)
-        for (int h = tid; h < a.H; h += kWarps * 32) a.lse[(long)h * a.T + t] = -INFINITY;
-    }
-  }
+  if (!open && tid == 0) ws.straddle[blockIdx.x].last = -1;
 }
 
-// One CTA per (CTA of the attention, row): where that CTA's last item goes on in the next ones, their
-// pieces of the row in list order.
+// One CTA per (CTA of the attention, query row): where that CTA's last item goes on in the next ones,
+// their pieces of the row in list order, one warp a piece at a time.
 constexpr int kCombineWarps = 8;
 
 template <int D, int NT>
 __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(AttnArgs a) {
   constexpr int kRows = 8 * NT, kPer = D / 32;
   __shared__ float part[kCombineWarps][D];
-  __shared__ float part_l[kCombineWarps];
+  __shared__ float part_ml[kCombineWarps][2];
   pdl_trigger();
   pdl_wait();
   const int cta = blockIdx.x, row = blockIdx.y, grid = gridDim.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Workspace ws = workspace_of(a.workspace, grid, Shape<D, NT>::kStreams, kRows, D);
   const Straddle st = ws.straddle[cta];
-  if (st.last < 0) return;
-  const int G = a.H / a.c.Hkv;
-  int first;
-  const int qn = q_tokens(a, st.b, first);
-  const int r = st.rt * kRows + row;
-  if (r >= qn * G) return;
-  const int last = st.last;
+  if (row >= st.rows || st.last < 0) return;
   auto at = [&](int w) { return ((size_t)w * 2 + (w == cta ? 1 : 0)) * kRows + row; };
-  float top = kNone;
-  for (int w = cta + lane; w <= last; w += 32) top = fmaxf(top, ws.ml[at(w) * 2]);
-  top = warp_max(top);
-  float acc[kPer], l = 0.f;
+  float acc[kPer], l = 0.f, top = kNone;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
 #pragma unroll 4
-  for (int w = cta + warp; w <= last; w += kCombineWarps) {
+  for (int w = cta + warp; w <= st.last; w += kCombineWarps) {
     const float2 ml = *reinterpret_cast<const float2*>(ws.ml + at(w) * 2);
-    const float e = fast_exp2(ml.x - top);
-    l = fmaf(e, ml.y, l);
     const float* o = ws.o + at(w) * D + lane * kPer;
+    float2 v[kPer / 2];
 #pragma unroll
-    for (int i = 0; i < kPer; i += 2) {
-      const float2 v = *reinterpret_cast<const float2*>(o + i);
-      acc[i] = fmaf(e, v.x, acc[i]);
-      acc[i + 1] = fmaf(e, v.y, acc[i + 1]);
+    for (int i = 0; i < kPer / 2; ++i) v[i] = reinterpret_cast<const float2*>(o)[i];
+    const float now = fmaxf(top, ml.x);
+    const float keep = fast_exp2(top - now), e = fast_exp2(ml.x - now);
+    top = now;
+    l = fmaf(e, ml.y, l * keep);
+#pragma unroll
+    for (int i = 0; i < kPer / 2; ++i) {
+      acc[2 * i] = fmaf(e, v[i].x, acc[2 * i] * keep);
+      acc[2 * i + 1] = fmaf(e, v[i].y, acc[2 * i + 1] * keep);
     }
   }
 #pragma unroll
   for (int i = 0; i < kPer; ++i) part[warp][lane * kPer + i] = acc[i];
-  if (lane == 0) part_l[warp] = l;
-  __syncthreads();
-  l = 0.f;
-  for (int w = 0; w < kCombineWarps; ++w) l += part_l[w];
-  const int qi = r / G, head = st.h * G + r % G;
-  if (threadIdx.x < D / 2) {
-    float v0 = 0.f, v1 = 0.f;
-#pragma unroll
-    for (int w = 0; w < kCombineWarps; ++w) {
-      v0 += part[w][2 * threadIdx.x];
-      v1 += part[w][2 * threadIdx.x + 1];
-    }
-    const float inv = row_inv(l);
-    reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.o) + ((long)(first + qi) * a.H + head) * D)[threadIdx.x] =
-        pack16(a.q_dtype, v0 * inv, v1 * inv);
+  if (lane == 0) {
+    part_ml[warp][0] = top;
+    part_ml[warp][1] = l;
   }
-  if (threadIdx.x == 0 && a.lse != nullptr) a.lse[(long)head * a.T + first + qi] = row_lse(top, l);
+  __syncthreads();
+  if (threadIdx.x >= D / 2) return;
+  top = kNone;
+  l = 0.f;
+  float v0 = 0.f, v1 = 0.f;
+#pragma unroll
+  for (int w = 0; w < kCombineWarps; ++w) top = fmaxf(top, part_ml[w][0]);
+#pragma unroll
+  for (int w = 0; w < kCombineWarps; ++w) {
+    const float e = fast_exp2(part_ml[w][0] - top);
+    l = fmaf(e, part_ml[w][1], l);
+    v0 = fmaf(e, part[w][2 * threadIdx.x], v0);
+    v1 = fmaf(e, part[w][2 * threadIdx.x + 1], v1);
+  }
+  const int G = a.H / a.c.Hkv, r = st.row0 + row, t = st.first + r / G, head = st.head + r % G;
+  const float inv = row_inv(l);
+  reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.o) + ((long)t * a.H + head) * D)[threadIdx.x] =
+      pack16(a.q_dtype, v0 * inv, v1 * inv);
+  if (threadIdx.x == 0 && a.lse != nullptr) a.lse[(long)head * a.T + t] = row_lse(top, l);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -869,15 +892,17 @@ template <int D, int NT, bool INT8>
 cudaError_t launch_attn(const AttnArgs& a, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t s) {
   using S = Shape<D, NT>;
   const size_t ring = 1024 + size_t(S::kStreams) * S::kRing + S::kQBytes;
-  const size_t smem = ring + size_t(a.B + 1) * sizeof(long long);
+  constexpr size_t kPerRequest = sizeof(long long) + 3 * sizeof(int);
+  const size_t smem = ring + size_t(a.B + 1) * kPerRequest;
   auto kernel = attn_kernel<D, NT, INT8>;
   cudaError_t e = once_per_device_kernel(reinterpret_cast<const void*>(kernel), [&] {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(ring + (kAttnMaxRows + 1) * sizeof(long long)));
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(ring + (kAttnMaxRows + 1) * kPerRequest));
   });
   if (e != cudaSuccess) return e;
   e = launch_pdl(kernel, dim3(unsigned(a.num_sms)), dim3(kWarps * 32), smem, s, km, vm, a);
   if (e != cudaSuccess) return e;
-  return launch_pdl(combine_kernel<D, NT>, dim3(unsigned(a.num_sms), S::kRows), dim3(kCombineWarps * 32), 0, s, a);
+  const long rows = std::min<long>((long)a.max_q * (a.H / a.c.Hkv), S::kRows);
+  return launch_pdl(combine_kernel<D, NT>, dim3(unsigned(a.num_sms), unsigned(rows)), dim3(kCombineWarps * 32), 0, s, a);
 }
 
 template <int D, int NT>
@@ -907,7 +932,7 @@ const char* attention(const AttnArgs& a, cudaStream_t s) {
   if (c.D != 64 && c.D != 128) return "attention_kv8: head_dim must be 64 or 128";
   if (c.P != 16 && c.P != 32 && c.P != 64 && c.P != 128) return "attention_kv8: page must be 16, 32, 64 or 128 tokens";
   if (a.H < 1 || c.Hkv < 1 || a.H % c.Hkv) return "attention_kv8: heads must be a multiple of the KV heads";
-  if (a.B > kAttnMaxRows) return "attention_kv8: at most 2048 requests";
+  if (a.B > kAttnMaxRows) return "attention_kv8: at most 1024 requests";
   if ((long)a.T * a.H > 0x7fffffffl || (long)a.max_q * a.H > 0x3fffffffl || (long)a.width * c.P > 0x7fffffc0l)
     return "attention_kv8: too many query rows or cached rows";
   if (c.page_stride % 16 || c.head_stride % 16 || c.token_stride % 16 || reinterpret_cast<uintptr_t>(c.k) % 16 ||

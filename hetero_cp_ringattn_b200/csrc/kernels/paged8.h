@@ -77,7 +77,7 @@ struct GatherArgs {
 };
 const char* gather(const GatherArgs& a, cudaStream_t s);
 
-constexpr int kAttnMaxRows = 2048;  // requests of one attention call
+constexpr int kAttnMaxRows = 1024;  // requests of one attention call
 
 struct AttnArgs {
   Cache c;

@@ -114,7 +114,7 @@ def attention_kv8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: to
     query token i of m sees rows 0 .. kv_len[b] - m + i. `max_q` bounds m. Returns (o [tokens, heads, D],
     lse [heads, tokens] natural log, or None); a token that sees no row gets o = 0, lse = -inf, so the
     partials of several ranks' shards merge like the other attention's (`reference.merge_partials`). At
-    most 2048 requests a call. Meant for decode steps and short segments (drafts to verify): for a long
+    most 1024 requests a call. Meant for decode steps and short segments (drafts to verify): for a long
     segment read the rows back with `gather_kv8` and use `kernels.attention`."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])

@@ -38,28 +38,32 @@ using namespace hcp::dev;
 
 namespace {
 
-constexpr int kWarps = 8;
 constexpr int kTile = 32;     // cached tokens a tile
 constexpr float kShift = 15.f;
 constexpr float kNone = -3e38f;   // the running maximum before any score (finite: differences stay numbers)
 constexpr float kLn2 = 0.6931471805599453f;
 
-// How the warps of a CTA share a tile stream. Up to 16 query rows (NT <= 2 column tiles): a stream a
-// warp, a tile at a time. More (NT = 3 or 5): two warps a stream, two tiles at a time; each computes
-// the scores of one tile, they exchange the column maxima and P, and each accumulates half of O's
-// dims over both tiles. So up to 40 rows take one pass over the cache with their accumulators in
-// registers, and no code is converted twice.
+// How the warps of a CTA share the tile streams. kTeam warps work on a stream, kStep tiles at a time:
+// each computes the scores of kMt 16-token groups, they exchange the column maxima and P, and each
+// accumulates kOut 16-dim pieces of O over all tokens of the step. So up to 40 query rows take one pass
+// over the cache with their accumulators in registers, no code is converted twice, and registers
+// allow the warps that hide each other's latencies (a warp alone issues about every fifth cycle).
 template <int D, int NT>
 struct Shape {
-  static constexpr bool kPair = NT > 2;
+  static constexpr int kTeam = NT <= 2 ? 1 : 2;
+  static constexpr int kStep = NT <= 2 ? 1 : 2;
+  static constexpr int kWarps = NT == 1 || (NT == 2 && D == 64) ? 12 : 8;
+  static constexpr int kThreads = kWarps * 32;
   static constexpr int kRows = 8 * NT;                      // query rows of an item
-  static constexpr int kStreams = kPair ? kWarps / 2 : kWarps;
+  static constexpr int kStreams = kWarps / kTeam;
+  static constexpr int kMt = 2 * kStep / kTeam;
+  static constexpr int kOut = D / 16 / kTeam;
   static constexpr int kBytes = 2 * kTile * D;              // K and V of a tile
-  // pair: q's fragments are read from shared memory (80 registers a lane for 40 rows of 128 dims)
-  static constexpr int kQBytes = kPair ? kStreams * kRows * D * 2 : 0;
-  static constexpr int kStages = (196608 - kQBytes) / (kStreams * kBytes);   // 192 KB: 3 to 10 stages
-  static constexpr int kStep = kPair ? 2 : 1;               // tiles a step
+  // a team reads q's fragments from shared memory (80 registers a lane for 40 rows of 128 dims)
+  static constexpr int kQBytes = kTeam > 1 ? kStreams * kRows * D * 2 : 0;
+  static constexpr int kStages = ((kTeam > 1 ? 176 : 192) * 1024 - kQBytes) / (kStreams * kBytes);
   static constexpr int kRing = kStages * kBytes;
+  static_assert(kMt >= 1 && kOut >= 2 && kOut % 2 == 0 && kStages >= 2 * kStep, "shape");
   static_assert(kRing >= kRows * D * 4, "a stream's last piece is left in its ring");
 };
 
@@ -181,43 +185,62 @@ struct Place {
   int n, qn, first;           // the request's cached rows, query tokens and the first of them
 };
 
+// A copying lane's next page, and its place in the list.
+struct CopyLane {
+  long long px;
+  Place pp;
+  int page, row, h;     // looked up: page id, first row in the page, KV head
+  int tile, valid;      // there is a tile; it reaches into this page
+};
+
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+
 // A finished row: o = acc / l, lse = (m - 15 + log2 l) ln 2; l = 0: the row saw nothing.
 __device__ __forceinline__ float row_lse(float m, float l) { return l == 0.f ? -INFINITY : (m - kShift + log2f(l)) * kLn2; }
 __device__ __forceinline__ float row_inv(float l) { return l == 0.f ? 0.f : __frcp_rn(l); }
 
-__device__ __forceinline__ void pair_sync(int pair) { asm volatile("bar.sync %0, 64;" ::"r"(pair + 1) : "memory"); }
+// The warps of a stream meet (named barrier 1 + stream).
+template <int TEAM>
+__device__ __forceinline__ void team_sync(int stream) {
+  if (TEAM == 1) __syncwarp();
+  else asm volatile("bar.sync %0, %1;" ::"r"(stream + 1), "n"(32 * TEAM) : "memory");
+}
 
 template <int D, int NT, bool INT8>
-__global__ void __launch_bounds__(kWarps * 32, 1)
+__global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1)
 attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, AttnArgs a) {
   using S = Shape<D, NT>;
-  constexpr bool kPair = S::kPair;
+  constexpr int kTeam = S::kTeam, kWarps = S::kWarps, kMt = S::kMt, kOut = S::kOut;
+  constexpr bool kShared = kTeam > 1;                      // q, maxima and P pass through shared memory
   constexpr int kStages = S::kStages, kBytes = S::kBytes, kRows = S::kRows, kStreams = S::kStreams, kStep = S::kStep;
   constexpr int kChunks = D / 16;                          // 16-dim pieces of a row
-  constexpr int kOut = kPair ? kChunks / 2 : kChunks;      // pieces of O a warp accumulates
   extern __shared__ unsigned char raw[];
   unsigned char* ring_base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  uint2* q_frag = reinterpret_cast<uint2*>(ring_base + kStreams * S::kRing);   // pair: [stream][piece][tile][lane]
+  uint2* q_frag = reinterpret_cast<uint2*>(ring_base + kStreams * S::kRing);   // team: [stream][piece][tile][lane]
   long long* prefix = reinterpret_cast<long long*>(ring_base + kStreams * S::kRing + S::kQBytes);
   int* s_rows = reinterpret_cast<int*>(prefix + a.B + 1);    // cached rows of each request
   int* s_first = s_rows + a.B;                               // its first query token, and (next B) their number
   __shared__ uint64_t bars[kStreams][kStages];
   __shared__ float meta[kStreams][kStages][2][2];          // k scale and v scale of the tile's (two) pages
+  __shared__ CopyLane s_copy[kStreams][2 * kStep];
   __shared__ long long warp_tot[kWarps];
   __shared__ float s_ml[kStreams][2][kRows][2];            // (m, l) of the streams' pieces
   __shared__ long long s_start[kStreams][2];               // first tile of the piece's item; -1: no piece
   __shared__ Place s_place[kStreams][2];
-  __shared__ float s_max[kPair ? kStreams : 1][2][kRows];  // pair: column maxima of the two warps
-  __shared__ uint32_t s_p[kPair ? kStreams : 1][2][kPair ? NT * 4 : 1][32];   // pair: their P^T fragments
+  __shared__ float s_max[kShared ? kStreams : 1][kTeam][kRows];   // team: the warps' column maxima
+  __shared__ uint32_t s_p[kShared ? kStreams : 1][2 * kStep][kShared ? NT * 2 : 1][32];   // team: P^T of each 16 tokens
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int stream = kPair ? warp >> 1 : warp, sub = kPair ? warp & 1 : 0;
+  const int stream = warp / kTeam, sub = warp % kTeam;
   const int G = a.H / a.c.Hkv, P = a.c.P, Hkv = a.c.Hkv;
   // a tile lies in one page of 32 tokens or more, or in two of 16
   const int halves = P == 16 ? 2 : 1;
   if (tid == 0) {
-    // a stage is full with its bytes (one arrival that announces them) and its pages' scales
+    // a stage is full with its pages' bytes and scales (a page's lane announces the bytes before it
+    // arrives with the scales, so the count cannot complete ahead of them)
     for (int w = 0; w < kStreams; ++w)
-      for (int i = 0; i < kStages; ++i) mbar_init(&bars[w][i], 1 + halves);
+      for (int i = 0; i < kStages; ++i) mbar_init(&bars[w][i], halves);
     fence_barrier_init();
     tma_prefetch_desc(&kmap);
     tma_prefetch_desc(&vmap);
@@ -288,70 +311,71 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
 
   // ---------------------------------------------------------------- the copies' side (one warp a stream)
   // One lane a page of up to kStep tiles (odd and even tiles of the range have lanes of their own); a
-  // page's id is looked up one turn ahead of its copies.
+  // page's id is looked up one turn ahead of its copies. The lanes' state lives in shared memory: it is
+  // needed once a step, and registers are what limits the number of warps.
   unsigned char* ring = ring_base + stream * S::kRing;
-  const int box = min(P, kTile);
-  const int my_tile = lane / halves, my_half = lane % halves;   // of the step (lanes past them: none)
   const bool copies = sub == 0;
-  long long px = x0 + my_tile;     // the lane's next tile
-  Place pp{};
-  int next_page = -1, next_row = 0, next_h = 0;
-  bool next_tile = false, next_valid = false;   // there is a tile; it reaches into the lane's page
-  int put_stage = 0, put_tile = 0;              // the next copy's stage, and its tile modulo kStep
-  auto look_up = [&] {
-    next_tile = my_tile < kStep && px < x1;
-    next_valid = false;
-    if (next_tile) {
-      const int block = pp.tile * kTile / P + my_half;
-      next_valid = block * P < pp.n;
-      if (next_valid) next_page = a.table[(long)pp.b * a.width + block];
-      next_row = pp.tile * kTile % P;
-      next_h = pp.h;
-      px += kStep;
-      pp.tile += kStep;
-      if (pp.tile >= pp.tiles && px < x1) pp = place_of(px);
+  auto look_up = [&](CopyLane& z, long long px, Place pp, int half) {
+    z.px = px;
+    z.tile = px < x1 ? 1 : 0;
+    z.valid = 0;
+    if (px < x1) {
+      const int block = pp.tile * kTile / P + half;
+      if (block * P < pp.n) {
+        z.valid = 1;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&z.page)), "l"(a.table + (long)pp.b * a.width + block)
+                     : "memory");
+      }
+      z.row = pp.tile * kTile % P;
+      z.h = pp.h;
     }
+    z.pp = pp;
   };
-  auto copy = [&](int tiles) {
+  auto copy = [&](int put_stage, int put_tile, int tiles) {
+    if (lane >= kStep * halves) return;
+    const int my_tile = lane / halves, my_half = lane % halves;
     const int ahead = my_tile >= put_tile ? my_tile - put_tile : my_tile - put_tile + kStep;
-    const bool turn = ahead < tiles;            // (lanes past kStep tiles have no tile)
-    int st = put_stage + ahead;
-    st = st >= kStages ? st - kStages : st;
-    const uint32_t valid = __ballot_sync(0xffffffffu, next_valid);
-    if (turn && next_tile) {
-      uint64_t* bar = &bars[stream][st];
-      if (my_half == 0) {
-        const uint32_t mine = (valid >> lane) & (halves == 2 ? 3u : 1u);
-        mbar_arrive_expect_tx(bar, uint32_t(__popc(mine)) * 2u * uint32_t(box) * D);
-      }
-      float* sc = meta[stream][st][my_half];
-      if (next_valid) {
-        unsigned char* dst = ring + st * kBytes + my_half * 16 * D;
-        // a page id outside the pool reads as zeros (the tensor map's bounds)
-        tma_load_4d(dst, &kmap, bar, next_row, next_h, next_page);
-        tma_load_4d(dst + kTile * D, &vmap, bar, next_row, next_h, next_page);
-      }
-      if (next_valid && next_page >= 0 && next_page < a.c.pages) {
-        const long at = (long)next_page * a.c.scale_page_stride + (long)next_h * a.c.scale_head_stride;
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(sc)), "l"(a.c.k_scale + at) : "memory");
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(sc + 1)), "l"(a.c.v_scale + at) : "memory");
-        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-      } else {
-        if (next_valid) report_error(a.status, int(StatusCode::kOutOfBounds), 411, next_page, next_h);
-        sc[0] = sc[1] = 1.f;
-        mbar_arrive(bar);
-      }
+    if (ahead >= tiles) return;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    CopyLane& z = s_copy[stream][lane];
+    if (!z.tile) return;
+    const int st = put_stage + ahead >= kStages ? put_stage + ahead - kStages : put_stage + ahead;
+    uint64_t* bar = &bars[stream][st];
+    const bool valid = z.valid != 0;
+    const int page = z.page;
+    // bytes of the lane's own page: the barrier counts the lanes
+    const int box = min(P, kTile);
+    float* sc = meta[stream][st][my_half];
+    if (valid) {
+      mbar_expect_tx(bar, 2u * uint32_t(box) * D);
+      unsigned char* dst = ring + st * kBytes + my_half * 16 * D;
+      // a page id outside the pool reads as zeros (the tensor map's bounds)
+      tma_load_4d(dst, &kmap, bar, z.row, z.h, page);
+      tma_load_4d(dst + kTile * D, &vmap, bar, z.row, z.h, page);
     }
-    if (turn) look_up();
-    put_stage += tiles;
-    put_stage = put_stage >= kStages ? put_stage - kStages : put_stage;
-    put_tile = (put_tile + tiles) % kStep;
+    if (valid && page >= 0 && page < a.c.pages) {
+      const long at = (long)page * a.c.scale_page_stride + (long)z.h * a.c.scale_head_stride;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(sc)), "l"(a.c.k_scale + at) : "memory");
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(sc + 1)), "l"(a.c.v_scale + at) : "memory");
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    } else {
+      if (valid) report_error(a.status, int(StatusCode::kOutOfBounds), 411, page, z.h);
+      sc[0] = sc[1] = 1.f;
+      mbar_arrive(bar);
+    }
+    const long long px = z.px + kStep;
+    Place pp = z.pp;
+    pp.tile += kStep;
+    if (pp.tile >= pp.tiles && px < x1) pp = place_of(px);
+    look_up(z, px, pp, my_half);
   };
   if (copies && x0 < x1) {
-    if (px < x1) pp = place_of(px);
-    look_up();
+    if (lane < kStep * halves) {
+      const long long px = x0 + lane / halves;
+      look_up(s_copy[stream][lane], px, px < x1 ? place_of(px) : Place{}, lane % halves);
+    }
 #pragma unroll 1
-    for (int i = 0; i < kStages; i += kStep) copy(min(kStep, kStages - i));
+    for (int i = 0; i < kStages; i += kStep) copy(i, 0, min(kStep, kStages - i));
   }
   __syncwarp();
 
@@ -378,7 +402,7 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
   const int out0 = sub * kOut;             // first piece of O of this warp
   int stage = 0;
   uint32_t phase = 0;                      // of `stage`; a stage before it in the ring is one phase on
-  int spent = 0;                           // pair mode: stages that take copies at the next step
+  int spent = 0, spent_at = 0, spent_tile = 0;   // team: stages that take copies at the next step
   long long x = x0;
   // A wait that ran out (reported) ends the waiting and the copies, not the loop: the barriers that two
   // warps share stay matched, and the rest of the range is computed on whatever the ring holds.
@@ -392,54 +416,58 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
 
     // q as the f16 B operand: lane (j, c) holds row j of each column tile, dims 16 s + 4 c .. + 3 of
     // k step s (the same order in which a lane's K bytes come out of ldmatrix)
-    uint32_t qf[kPair ? 1 : NT][kPair ? 1 : kChunks][2];
+    uint32_t qf[kShared ? 1 : NT][kShared ? 1 : kChunks][2];
     uint2* qs = q_frag + stream * kChunks * NT * 32 + lane;
-    float f[NT][2];          // score factor of the lane's two columns
-    int lim[NT][2];          // rows seen by them
     float m[NT][2], l[NT][2];
     float acc[kOut][NT][4];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
+    const uint16_t* q_at = reinterpret_cast<const uint16_t*>(a.q) + (long)p.first * a.q_stride + (long)p.h * G * a.q_head_stride + 4 * c;
+    auto load_q = [&](int t, float (&v)[kChunks][4]) {
       const int r = t * 8 + j;
-      float v[kChunks][4];
-      float top = 0.f;
-      const bool have = r < rows;
       const int qi = (r0 + r) / G, g = (r0 + r) % G;
-      const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (long)(p.first + qi) * a.q_stride +
-                            (long)(p.h * G + g) * a.q_head_stride + 4 * c;
+      const uint16_t* src = q_at + (long)qi * a.q_stride + (long)g * a.q_head_stride;
 #pragma unroll
       for (int s = 0; s < kChunks; ++s) {
-        const uint2 w = have ? *reinterpret_cast<const uint2*>(src + 16 * s) : make_uint2(0, 0);
+        const uint2 w = r < rows ? *reinterpret_cast<const uint2*>(src + 16 * s) : make_uint2(0, 0);
         if (a.q_dtype == kBF16) {
           v[s][0] = bf16_lo(w.x); v[s][1] = bf16_hi(w.x); v[s][2] = bf16_lo(w.y); v[s][3] = bf16_hi(w.y);
         } else {
           const float2 lo = half2_floats(w.x), hi = half2_floats(w.y);
           v[s][0] = lo.x; v[s][1] = lo.y; v[s][2] = hi.x; v[s][3] = hi.y;
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(v[s][i]));
       }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // |q| 2^e in [2^14, 2^15) for the row's largest element
-      const int e = top > 0.f ? max(-113, min(100, 14 - (((__float_as_int(top) >> 23) & 0xff) - 127))) : 0;
-      const float up = pow2(e);
+    };
+    // |q| 2^e in [2^14, 2^15) for the item's largest finite element: bf16's 8 bits stay exact in f16
+    // down to 2^-32 of it
+    float top_q = 0.f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float v[kChunks][4];
+      load_q(t, v);
+#pragma unroll
+      for (int s = 0; s < kChunks; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top_q = fmaxf(top_q, fabsf(v[s][i]) < 3.4e38f ? fabsf(v[s][i]) : 0.f);
+    }
+    top_q = warp_max(top_q);
+    const int e2 = top_q > 0.f ? max(-113, min(100, 14 - (((__float_as_int(top_q) >> 23) & 0xff) - 127))) : 0;
+    const float factor = a.scale * 1.4426950408889634f * pow2(-e2);   // of the scores, to the log2 domain
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float v[kChunks][4];
+      load_q(t, v);
+      const float up = pow2(e2);
 #pragma unroll
       for (int s = 0; s < kChunks; ++s) {
         const uint32_t lo = pack_half(v[s][0] * up, v[s][1] * up), hi = pack_half(v[s][2] * up, v[s][3] * up);
-        if constexpr (kPair) {
-          if (sub == (t & 1)) qs[(s * NT + t) * 32] = make_uint2(lo, hi);
+        if constexpr (kShared) {
+          if (sub == t % kTeam) qs[(s * NT + t) * 32] = make_uint2(lo, hi);
         } else {
           qf[t][s][0] = lo;
           qf[t][s][1] = hi;
         }
       }
-      const float back = a.scale * 1.4426950408889634f * pow2(-e);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        f[t][i] = __shfl_sync(0xffffffffu, back, (2 * c + i) * 4);
-        const int col = t * 8 + 2 * c + i;
-        lim[t][i] = col < rows ? n - qn + (r0 + col) / G + 1 : n;
         m[t][i] = kNone;
         l[t][i] = 0.f;
       }
@@ -448,7 +476,7 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[s][t][i] = 0.f;
     }
-    if (kPair) pair_sync(stream);
+    if (kShared) team_sync<kTeam>(stream);
     const int qi0 = r0 / G, qi1 = (r0 + rows - 1) / G;    // the item's query tokens
     const int least = n - qn + qi0 + 1;                   // rows that all of them see
 
@@ -460,15 +488,16 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
       const int base = tile * kTile;
       const uint32_t ring_at = smem_u32(ring);
       const bool edge = base + kStep * kTile > least || count < kStep;
-      const bool idle = sub >= count;                     // no tile for this warp in this step
-      const int k_stage = stage_at(sub);
-      const uint32_t kbase = ring_at + k_stage * kBytes;
-      // ---- S^T = K Q^T of this warp's tile
-      float s[2][NT][4];
-      float iv[2];
-      bool dead[2];
+      // ---- S^T = K Q^T of this warp's 16-token groups: group g is half g % 2 of the step's tile g / 2
+      const int g0 = sub * kMt;
+      const bool idle = g0 / 2 >= count;                  // its tile is not there in this step
+      const int k_stage = stage_at(g0 / 2);
+      const uint32_t kbase = ring_at + k_stage * kBytes + (kMt == 2 ? 0 : (g0 & 1) * 16 * D);
+      float s[kMt][NT][4];
+      float iv[kMt];
+      bool dead[kMt];
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
+      for (int mt = 0; mt < kMt; ++mt)
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -480,11 +509,11 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            if constexpr (kPair) qb[h][t] = qs[((k + h) * NT + t) * 32];
+            if constexpr (kShared) qb[h][t] = qs[((k + h) * NT + t) * 32];
             else qb[h][t] = make_uint2(qf[t][k + h][0], qf[t][k + h][1]);
           }
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
+        for (int mt = 0; mt < kMt; ++mt) {
           uint32_t r[4];
           ldmatrix4(kbase + piece<D>(mt * 16 + (lane & 15), k + (lane >> 4)), r);
 #pragma unroll
@@ -499,54 +528,61 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
       }
       // ---- in the log2 domain, masked; the running maximum
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        const int half = halves == 2 ? mt : 0;
+      for (int mt = 0; mt < kMt; ++mt) {
+        const int half = halves == 2 ? (g0 + mt) & 1 : 0;
         const float ks = meta[stream][k_stage][half][0], vs = meta[stream][k_stage][half][1];
         // a block scaled by 0 holds zeros: its weight counts in l and its p V is 0 whatever p is
         dead[mt] = vs == 0.f || idle;
         const float lv = dead[mt] ? 0.f : __log2f(vs);
         iv[mt] = dead[mt] ? 1.f : __fdividef(1.f, vs);
+        const float f = factor * ks;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const float f0 = f[t][0] * ks, f1 = f[t][1] * ks;
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[mt][t][i] = fmaf(s[mt][t][i], i & 1 ? f1 : f0, lv);
-        }
+          for (int i = 0; i < 4; ++i) s[mt][t][i] = fmaf(s[mt][t][i], f, lv);
       }
       if (edge) {
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int t = 0; t < NT; ++t)
+          for (int i = 0; i < 4; ++i) {
+            // rows that query row t * 8 + 2 c + (i & 1) sees (past the item's rows: any)
+            const int col = t * 8 + 2 * c + (i & 1);
+            const int lim = idle ? 0 : col < rows ? n - qn + (r0 + col) / G + 1 : n;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (idle || base + sub * kTile + mt * 16 + j + (i >> 1) * 8 >= lim[t][i & 1]) s[mt][t][i] = -INFINITY;
+            for (int mt = 0; mt < kMt; ++mt)
+              if (base + (g0 + mt) * 16 + j + (i >> 1) * 8 >= lim) s[mt][t][i] = -INFINITY;
+          }
       }
       float top[NT][2];
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float v = fmaxf(fmaxf(s[0][t][i], s[0][t][i + 2]), fmaxf(s[1][t][i], s[1][t][i + 2]));
+          float v = fmaxf(s[0][t][i], s[0][t][i + 2]);
+#pragma unroll
+          for (int mt = 1; mt < kMt; ++mt) v = fmaxf(v, fmaxf(s[mt][t][i], s[mt][t][i + 2]));
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
           top[t][i] = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
         }
-      if (kPair) {
+      if (kShared) {
         if (j == 0) {
 #pragma unroll
           for (int t = 0; t < NT; ++t)
             *reinterpret_cast<float2*>(&s_max[stream][sub][t * 8 + 2 * c]) = make_float2(top[t][0], top[t][1]);
         }
-        pair_sync(stream);
-        // both warps are past the previous step: its stages take the next copies
-        if (copies && alive && spent > 0) copy(spent);
+        team_sync<kTeam>(stream);
+        // all warps are past the previous step: its stages take the next copies
+        if (copies && alive && spent > 0) copy(spent_at, spent_tile, spent);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const float2 o = *reinterpret_cast<const float2*>(&s_max[stream][sub ^ 1][t * 8 + 2 * c]);
-          top[t][0] = fmaxf(top[t][0], o.x);
-          top[t][1] = fmaxf(top[t][1], o.y);
-        }
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int o = 1; o < kTeam; ++o) {
+            const float2 v = *reinterpret_cast<const float2*>(&s_max[stream][sub ^ o][t * 8 + 2 * c]);
+            top[t][0] = fmaxf(top[t][0], v.x);
+            top[t][1] = fmaxf(top[t][1], v.y);
+          }
       }
       bool changed = false;
 #pragma unroll
@@ -568,13 +604,13 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
             for (int i = 0; i < 4; ++i) acc[k][t][i] *= up[i & 1];
         }
       }
-      // ---- p, its sum, and P^T as the B operand of the tile's two 16-token steps
-      uint32_t pf[2][NT][2];
+      // ---- p, its sum, and P^T as the B operand of a 16-token step
+      uint32_t pf[kMt][NT][2];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const float mu[2] = {m[t][0] - kShift, m[t][1] - kShift};
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
+        for (int mt = 0; mt < kMt; ++mt) {
           float e[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -584,17 +620,13 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
           const uint32_t lo = pack_half(e[0], e[1]), hi = pack_half(e[2], e[3]);
           pf[mt][t][0] = transpose8x8(dead[mt] ? 0u : lo);
           pf[mt][t][1] = transpose8x8(dead[mt] ? 0u : hi);
+          if constexpr (kShared) {
+            s_p[stream][g0 + mt][2 * t][lane] = pf[mt][t][0];
+            s_p[stream][g0 + mt][2 * t + 1][lane] = pf[mt][t][1];
+          }
         }
       }
-      if (kPair) {
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) s_p[stream][sub][(mt * NT + t) * 2 + i][lane] = pf[mt][t][i];
-        pair_sync(stream);
-      }
+      if (kShared) team_sync<kTeam>(stream);
       // ---- O^T += V^T P^T. In a step that ends inside the rows some query token sees, every query
       // token gets a pass of its own with the codes it must not see taken as 0: whatever a masked
       // place holds (stale bytes behind the end, NaN in a later draft's row), p = 0 cannot cancel it.
@@ -605,9 +637,9 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
           uint32_t b0[NT], b1[NT];
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            if constexpr (kPair) {
-              b0[t] = s_p[stream][q][(mt * NT + t) * 2][lane];
-              b1[t] = s_p[stream][q][(mt * NT + t) * 2 + 1][lane];
+            if constexpr (kShared) {
+              b0[t] = s_p[stream][q * 2 + mt][2 * t][lane];
+              b1[t] = s_p[stream][q * 2 + mt][2 * t + 1][lane];
             } else {
               b0[t] = pf[mt][t][0];
               b1[t] = pf[mt][t][1];
@@ -651,13 +683,18 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
             if (seen > base + q * kTile) values(q, seen, false);
         }
       }
-      // ---- the stages are free (pair mode: once the other warp is known to be done with them, at the
+      // ---- the stages are free (team: once the other warps are known to be done with them, at the
       // next step's first barrier)
-      spent = count;
+      if (kShared) {
+        spent_at = stage;
+        // stage i of the prologue took tile i of the range, so a copy's tile modulo kStep follows
+        spent_tile = int(x - x0 + kStages) % kStep;
+        spent = count;
+      }
       x += count;
-      if (!kPair) {
+      if (!kShared) {
         __syncwarp();
-        if (alive) copy(1);
+        if (alive) copy(stage, 0, 1);
       }
       stage += count;
       if (stage >= kStages) {
@@ -675,22 +712,25 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
         v += __shfl_xor_sync(0xffffffffu, v, 8);
         l[t][i] = v + __shfl_xor_sync(0xffffffffu, v, 16);
       }
-    if (kPair) {   // each warp has the sums of its own tokens
-      pair_sync(stream);
+    if (kShared) {   // each warp has the sums of its own tokens
+      team_sync<kTeam>(stream);
       if (j == 0) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
           *reinterpret_cast<float2*>(&s_max[stream][sub][t * 8 + 2 * c]) = make_float2(l[t][0], l[t][1]);
       }
-      pair_sync(stream);
+      team_sync<kTeam>(stream);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const float2 o0 = *reinterpret_cast<const float2*>(&s_max[stream][0][t * 8 + 2 * c]);
-        const float2 o1 = *reinterpret_cast<const float2*>(&s_max[stream][1][t * 8 + 2 * c]);
-        l[t][0] = o0.x + o1.x;
-        l[t][1] = o0.y + o1.y;
+        l[t][0] = l[t][1] = 0.f;
+#pragma unroll
+        for (int o = 0; o < kTeam; ++o) {
+          const float2 v = *reinterpret_cast<const float2*>(&s_max[stream][o][t * 8 + 2 * c]);
+          l[t][0] += v.x;
+          l[t][1] += v.y;
+        }
       }
-      pair_sync(stream);
+      team_sync<kTeam>(stream);
     }
     const bool complete = p.tile == 0 && end == p.tiles;
     const bool last = x >= x1;
@@ -711,7 +751,7 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
           }
         }
     } else {
-      // the range's last piece stays in the stream's ring (free: all its tiles are consumed; the pair
+      // the range's last piece stays in the stream's ring (free: all its tiles are consumed; the team
       // has just met), a first piece before another item goes to the workspace
       const int slot = last ? 1 : 0;
       float* po = last ? reinterpret_cast<float*>(ring) : ws.head + ((size_t)blockIdx.x * kStreams + stream) * kRows * D;
@@ -899,7 +939,7 @@ cudaError_t launch_attn(const AttnArgs& a, const CUtensorMap& km, const CUtensor
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(ring + (kAttnMaxRows + 1) * kPerRequest));
   });
   if (e != cudaSuccess) return e;
-  e = launch_pdl(kernel, dim3(unsigned(a.num_sms)), dim3(kWarps * 32), smem, s, km, vm, a);
+  e = launch_pdl(kernel, dim3(unsigned(a.num_sms)), dim3(S::kThreads), smem, s, km, vm, a);
   if (e != cudaSuccess) return e;
   const long rows = std::min<long>((long)a.max_q * (a.H / a.c.Hkv), S::kRows);
   return launch_pdl(combine_kernel<D, NT>, dim3(unsigned(a.num_sms), unsigned(rows)), dim3(kCombineWarps * 32), 0, s, a);
@@ -924,7 +964,10 @@ cudaError_t attn_rows(const AttnArgs& a, const CUtensorMap& km, const CUtensorMa
 
 size_t attention_workspace(const AttnArgs& a) {
   const int nt = column_tiles(a);
-  return workspace_of(nullptr, a.num_sms, nt > 2 ? kWarps / 2 : kWarps, 8 * nt, a.c.D).bytes;
+  auto bytes = [&](auto shape) { return workspace_of(nullptr, a.num_sms, shape.kStreams, shape.kRows, a.c.D).bytes; };
+  if (a.c.D == 64)
+    return nt == 1 ? bytes(Shape<64, 1>{}) : nt == 2 ? bytes(Shape<64, 2>{}) : nt == 3 ? bytes(Shape<64, 3>{}) : bytes(Shape<64, 5>{});
+  return nt == 1 ? bytes(Shape<128, 1>{}) : nt == 2 ? bytes(Shape<128, 2>{}) : nt == 3 ? bytes(Shape<128, 3>{}) : bytes(Shape<128, 5>{});
 }
 
 const char* attention(const AttnArgs& a, cudaStream_t s) {

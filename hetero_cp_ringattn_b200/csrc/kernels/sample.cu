@@ -15,10 +15,13 @@
 // are 0; u has 24 bits and cannot reach them.
 //
 // One cluster per row: each CTA holds a contiguous slice of the row in shared memory, so the logits
-// are read from memory once. The k-th and the top-p cut are found by a histogram over d (bins of
-// 1/64, counts and weight sums, summed over the cluster through distributed shared memory), then
-// exactly among the few tokens of the crossing bin. Bound: the chain of block and cluster barriers
-// for a few rows, the shared-memory passes and atomics for many.
+// are read from memory once. A histogram over d (bins of 1/64; counts and weight sums of the tokens
+// near the maximum, of all of them only if the cut lies further out) gives the bin where the cut
+// falls; the tokens up to it, usually a few dozen, are gathered into one CTA, sorted and finished
+// there. More than 1024 of them (a large k, a flat row, ties) take the general way: histograms of the
+// crossing bin until it is small, or the exact tie, then one pass over the kept tokens.
+// Bound: instructions per token (distance, weight) for many rows, the chain of cluster barriers for
+// one. The weight's polynomial runs on packed pairs.
 #include <cooperative_groups.h>
 
 #include <cuda_bf16.h>
@@ -40,17 +43,13 @@ typedef unsigned long long u64;
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
-constexpr int kList = 512;          // tokens of a crossing bin that are ordered directly
+constexpr int kList = 1024;         // tokens that are ordered directly (one a thread)
+constexpr int kNear = 640;          // bins of the first histogram: d < 10
 constexpr int kMaxCluster = 16;     // 16 is the hardware's limit (above 8: opt-in)
 constexpr int kMaxSlice = 45056;    // floats of a row in one CTA's shared memory
 constexpr u64 kAll = ~0ull;
 
 // The fixed operations of the weight: no contraction, no flush of subnormals, whatever the flags.
-__device__ __forceinline__ float mul_rn(float a, float b) {
-  float r;
-  asm("mul.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 __device__ __forceinline__ float add_rn(float a, float b) {
   float r;
   asm("add.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -63,25 +62,35 @@ __device__ __forceinline__ float div_rn(float a, float b) {
 }
 
 // floor(2^31 exp(-d)) for 0 <= d <= 64: y = d log2(e), n = round(y), 2^(n - y) on [-1/2, 1/2] by the
-// Taylor series of 2^g to degree 7 (remainder below 1e-8), then a shift by n.
-__device__ __forceinline__ uint32_t weight(float d) {
-  const float y = mul_rn(d, 0x1.715476p+0f);
-  const float n = rintf(y);
-  const float g = add_rn(n, -y);
-  float w = 0x1.ffcbfcp-17f;
-  w = add_rn(mul_rn(w, g), 0x1.430912p-13f);
-  w = add_rn(mul_rn(w, g), 0x1.5d87fep-10f);
-  w = add_rn(mul_rn(w, g), 0x1.3b2ab6p-7f);
-  w = add_rn(mul_rn(w, g), 0x1.c6b08ep-5f);
-  w = add_rn(mul_rn(w, g), 0x1.ebfbep-3f);
-  w = add_rn(mul_rn(w, g), 0x1.62e43p-1f);
-  w = add_rn(mul_rn(w, g), 1.0f);
-  const uint32_t fix = __float2uint_rz(w * 2147483648.f);
-  const int sh = int(n);
-  return sh > 31 ? 0u : fix >> sh;
+// Taylor series of 2^g to degree 7 (remainder below 1e-8), then a shift by n. Adding and subtracting
+// 1.5 * 2^23 rounds y to the nearest integer (ties to even) and leaves it in the sum's low bits.
+__device__ __forceinline__ uint2 weight2(float d0, float d1) {
+  auto pair = [](float x) { return make_float2(x, x); };
+  const float2 y = __fmul2_rn(make_float2(d0, d1), pair(0x1.715476p+0f));
+  const float2 t = __fadd2_rn(y, pair(12582912.f));
+  const float2 n = __fadd2_rn(t, pair(-12582912.f));
+  const float2 g = __fadd2_rn(n, make_float2(-y.x, -y.y));
+  float2 w = __fadd2_rn(__fmul2_rn(pair(0x1.ffcbfcp-17f), g), pair(0x1.430912p-13f));
+  w = __fadd2_rn(__fmul2_rn(w, g), pair(0x1.5d87fep-10f));
+  w = __fadd2_rn(__fmul2_rn(w, g), pair(0x1.3b2ab6p-7f));
+  w = __fadd2_rn(__fmul2_rn(w, g), pair(0x1.c6b08ep-5f));
+  w = __fadd2_rn(__fmul2_rn(w, g), pair(0x1.ebfbep-3f));
+  w = __fadd2_rn(__fmul2_rn(w, g), pair(0x1.62e43p-1f));
+  w = __fadd2_rn(__fmul2_rn(w, g), pair(1.0f));
+  // w in (0.7, 1.42): 24 significant bits at 2^-23 or 2^-24 (one place further down)
+  auto fixed = [](float v, float sum) {
+    const uint32_t b = __float_as_uint(v);
+    const int sh = int(__float_as_uint(sum) & 0x7f) + int(127 - (b >> 23));
+    return sh > 31 ? 0u : ((b << 8) | 0x80000000u) >> sh;
+  };
+  return make_uint2(fixed(w.x, t.x), fixed(w.y, t.y));
 }
+__device__ __forceinline__ uint32_t weight(float d) { return weight2(d, d).x; }
 
-__device__ __forceinline__ int bin_of(float d) { return min(int(d * 64.f), kBins - 1); }
+// floor(64 d), at most kBins - 1 (d <= 64: adding 2^23 towards zero leaves the floor in the low bits).
+__device__ __forceinline__ int bin_of(float d) {
+  return min(int(__float_as_uint(__fadd_rz(d * 64.f, 8388608.f)) & 0x7fffff), kBins - 1);
+}
 
 // floor(total * x) for x in [0, 1], x held in 24 bits (total < 2^54).
 __device__ __forceinline__ u64 share(u64 total, float x) {
@@ -96,18 +105,50 @@ __device__ __forceinline__ u64 warp_sum64(u64 v) {
   return v;
 }
 
-struct Shared {
-  uint32_t cnt[kBins], wlo[kBins], whi[kBins];   // this CTA's histogram
-  u64 list[kList];                               // this CTA's tokens of the crossing bin
+__device__ __forceinline__ u64 warp_scan64(u64 v, int lane) {   // inclusive
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const u64 up = __shfl_up_sync(0xffffffffu, v, d);
+    if (lane >= d) v += up;
+  }
+  return v;
+}
+
+struct __align__(16) Shared {
+  // this CTA's histogram: x: count in the low 16 bits, carries of y in the high ones; y: weights
+  // modulo 2^32 (a slice has at most 45056 tokens of at most 2^31, so both halves hold)
+  uint2 hist[kBins];
+  u64 list[kList];                               // this CTA's gathered tokens, (key, index)
   u64 all[kList];                                // the cluster's
   u64 warp_a[kWarps], warp_b[kWarps];
   u64 slot[2][kMaxCluster];                      // one value of every CTA, pushed by it
   float fslot[kMaxCluster];
   int list_n;
   u64 found;                                     // results one thread hands to the block
-  u64 found_cnt, found_w, found_in_cnt, found_in_w;
+  u64 found_cnt, found_w, found_in_cnt;
   int found_bin;
 };
+
+// Ascending bitonic sort of one u64 a thread, `size` a power of two of threads (the rest idle along).
+// Exchanges within a warp are shuffles, wider ones go through `buf`.
+__device__ __forceinline__ u64 sort64(u64 v, int size, u64* buf, int tid) {
+  for (int k = 2; k <= size; k <<= 1) {
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      u64 o;
+      if (j >= 32) {
+        __syncthreads();
+        if (tid < size) buf[tid] = v;
+        __syncthreads();
+        o = tid < size ? buf[tid ^ j] : 0;
+      } else {
+        o = __shfl_xor_sync(0xffffffffu, v, j);
+      }
+      const bool low = (tid & j) == 0, up = (tid & k) == 0;
+      if (tid < size) v = (low == up) ? (o < v ? o : v) : (o > v ? o : v);
+    }
+  }
+  return v;
+}
 
 template <bool BF16>
 __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a, int slice) {
@@ -167,9 +208,10 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a, int s
   const bool greedy = !(temp > 0.f);
   const bool use_k = !greedy && top_k > 0 && top_k < a.V;
   const bool use_p = !greedy && top_p > 0.f && top_p < 1.f;
-  if (use_k || use_p) {
-    for (int i = tid; i < kBins; i += kThreads) S.cnt[i] = S.wlo[i] = S.whi[i] = 0;
-  }
+  auto clear = [&] {
+    for (int i = tid; i < kBins; i += kThreads) S.hist[i] = make_uint2(0, 0);
+  };
+  if (use_k || use_p) clear();
   if (tid == 0) S.list_n = 0;
   top = warp_max(top);
   float* wf = reinterpret_cast<float*>(S.warp_a);
@@ -209,300 +251,327 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a, int s
 
   // ---------------------------------------------------------------- distances, totals, histogram
   auto add_to_bin = [&](int bin, uint32_t w) {
-    atomicAdd(&S.cnt[bin], 1u);
+    uint32_t one = 1;
     if (w) {
-      const uint32_t was = atomicAdd(&S.wlo[bin], w);
-      if (was + w < was) atomicAdd(&S.whi[bin], 1u);   // the carry of a 64-bit sum
+      const uint32_t was = atomicAdd(&S.hist[bin].y, w);
+      if (was + w < was) one += 0x10000u;     // the carry of a 64-bit sum
     }
+    atomicAdd(&S.hist[bin].x, one);
   };
-  u64 sum = 0;
-  for (int i = s0 + lane; i < s1; i += 32) {
-    const float l = x[i];
-    float d = l == top ? 0.f : div_rn(top - l, temp);
-    d = d == d ? fminf(d, 64.f) : 64.f;
-    x[i] = d;
-    const uint32_t w = weight(d);
-    sum += w;
-    if (use_k || use_p) add_to_bin(bin_of(d), w);
-  }
-
-  u64 cut = kAll;
-  if (use_k || use_p) {
-    const uint32_t* xkey = reinterpret_cast<const uint32_t*>(x);
-    // Finds the (key, index) of the last kept token of a prefix search, the prefix's weight
-    // included in `kept_w`. Levels: the histogram in place covers keys [key_lo, key_hi] with
-    // `shift` (the first level: d in bins of 1/64); a crossing bin of at most kList tokens is
-    // ordered directly, a larger one gets a histogram of its own.
-    u64 limit_id = kAll;     // top-p looks at the tokens that top-k kept
-    bool dirty = false;      // the first level's histogram has been overwritten
-    auto publish = [&] { cluster.sync(); };
-    auto find_bin = [&](bool by_weight, u64 target, u64 base_cnt, u64 base_w) {
-      // sums of two bins a thread over the cluster, then a block scan to the crossing bin
-      u64 c[2] = {0, 0}, w[2] = {0, 0};
-      for (int r = 0; r < C; ++r) {
-        const Shared* o = cluster.map_shared_rank(&S, r);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int bin = 2 * tid + j;
-          c[j] += o->cnt[bin];
-          w[j] += (u64(o->whi[bin]) << 32) + o->wlo[bin];
-        }
-      }
-      u64 ic = c[0] + c[1], iw = w[0] + w[1];
-      const u64 oc = ic, ow = iw;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const u64 uc = __shfl_up_sync(0xffffffffu, ic, d), uw = __shfl_up_sync(0xffffffffu, iw, d);
-        if (lane >= d) {
-          ic += uc;
-          iw += uw;
-        }
-      }
-      if (tid == 0) S.found_bin = -1;
-      if (lane == 31) {
-        S.warp_a[warp] = ic;
-        S.warp_b[warp] = iw;
-      }
-      __syncthreads();
-      u64 ec = base_cnt + ic - oc, ew = base_w + iw - ow;
-      for (int i = 0; i < warp; ++i) {
-        ec += S.warp_a[i];
-        ew += S.warp_b[i];
-      }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const u64 before = by_weight ? ew : ec, in = by_weight ? w[j] : c[j];
-        if (before < target && before + in >= target) {
-          S.found_bin = 2 * tid + j;
-          S.found_cnt = ec;
-          S.found_w = ew;
-          S.found_in_cnt = c[j];
-          S.found_in_w = w[j];
-        }
-        ec += c[j];
-        ew += w[j];
-      }
-      __syncthreads();
-    };
-    // Among the tokens whose key lies in [key_lo, key_hi] (all of them in the list): the last
-    // kept one. `before`: count or weight ahead of the list.
-    auto order_list = [&](uint32_t key_lo, uint32_t key_hi, bool by_weight, u64 target, u64 base_cnt, u64 base_w,
-                          u64& kept_w) {
-      for (int i = s0 + lane; i < s1; i += 32) {
-        const uint32_t key = xkey[i];
-        if (key >= key_lo && key <= key_hi) {
-          const int at = atomicAdd(&S.list_n, 1);
-          if (at < kList) S.list[at] = (u64(key) << 32) | uint32_t(lo + i);
-        }
-      }
-      publish();
-      int total = 0;
-      for (int r = 0; r < C; ++r) {
-        const Shared* o = cluster.map_shared_rank(&S, r);
-        const int m = min(o->list_n, kList);
-        for (int i = tid; i < m && total + i < kList; i += kThreads) S.all[total + i] = o->list[i];
-        total = min(total + m, kList);
-      }
-      if (tid == 0) {
-        S.found = kAll;
-        S.found_w = 0;
-      }
-      __syncthreads();
-      // one thread a token: what is ahead of it decides
-      if (tid < total) {
-        const u64 me = S.all[tid];
-        u64 cnt = base_cnt, w = base_w;
-        for (int i = 0; i < total; ++i) {
-          const u64 o = S.all[i];
-          if (o < me) {
-            ++cnt;
-            w += weight(__uint_as_float(uint32_t(o >> 32)));
-          }
-        }
-        const u64 own = weight(__uint_as_float(uint32_t(me >> 32)));
-        const u64 before = by_weight ? w : cnt, in = by_weight ? own : 1;
-        if (before < target && before + in >= target) {
-          S.found = me;
-          S.found_w = w + own;
-        }
-      }
-      publish();             // also: every CTA has read the lists
-      if (tid == 0) S.list_n = 0;
-      kept_w = S.found_w;
-      const u64 id = S.found;
-      __syncthreads();
-      return id;
-    };
-    // The crossing bin at `shift` levels below the first; fills a new histogram of [key_lo, key_hi].
-    auto refine = [&](uint32_t key_lo, uint32_t key_hi, bool by_weight, u64 target, u64 base_cnt, u64 base_w,
-                      u64 in_cnt, u64& kept_w) -> u64 {
-      while (true) {
-        if (in_cnt <= kList) return order_list(key_lo, key_hi, by_weight, target, base_cnt, base_w, kept_w);
-        if (key_lo == key_hi) {
-          // more equal keys than the list holds: the m-th of them in index order is the last kept
-          const uint32_t w = weight(__uint_as_float(key_lo));
-          u64 m = by_weight ? (target - base_w + w - 1) / max(w, 1u) : target - base_cnt;
-          kept_w = base_w + m * w;
-          u64 cnt = 0;
-          for (int i = s0 + lane; i < s1; i += 32) cnt += xkey[i] == key_lo;
-          cnt = warp_sum64(cnt);
-          if (lane == 0) S.warp_a[warp] = cnt;
-          __syncthreads();
-          if (tid == 0) {
-            u64 t = 0;
-            for (int i = 0; i < kWarps; ++i) t += S.warp_a[i];
-            for (int r = 0; r < C; ++r) *cluster.map_shared_rank(&S.slot[1][rank], r) = t;
-          }
-          publish();
-          u64 ahead = 0, mine = 0;
-          int owner = C - 1;
-          for (int r = 0; r < C; ++r) {
-            if (ahead + S.slot[1][r] >= m) {
-              owner = r;
-              break;
-            }
-            ahead += S.slot[1][r];
-          }
-          mine = ahead;
-          if (owner == rank) {
-            for (int i = 0; i < warp; ++i) mine += S.warp_a[i];
-            if (mine < m && mine + S.warp_a[warp] >= m) {
-              for (int base = s0; base < s1; base += 32) {
-                const int i = base + lane;
-                const uint32_t hit = __ballot_sync(0xffffffffu, i < s1 && xkey[i] == key_lo);
-                const int c = __popc(hit);
-                if (mine + c >= m) {
-                  const int nth = int(m - mine);   // 1-based among the hits of these 32
-                  if ((hit >> lane & 1) && __popc(hit & ((2u << lane) - 1)) == nth) {
-                    const u64 id = (u64(key_lo) << 32) | uint32_t(lo + i);
-                    for (int r = 0; r < C; ++r) *cluster.map_shared_rank(&S.found, r) = id;
-                  }
-                  break;
-                }
-                mine += c;
-              }
-            }
-          }
-          publish();
-          const u64 id = S.found;
-          publish();
-          return id;
-        }
-        publish();           // every CTA has read the previous histogram
-        dirty = true;
-        for (int i = tid; i < kBins; i += kThreads) S.cnt[i] = S.wlo[i] = S.whi[i] = 0;
-        __syncthreads();
-        int shift = 0;
-        while (((key_hi - key_lo) >> shift) >= kBins) ++shift;
-        for (int i = s0 + lane; i < s1; i += 32) {
-          const uint32_t key = xkey[i];
-          if (key >= key_lo && key <= key_hi) {
-            add_to_bin((key - key_lo) >> shift, weight(x[i]));
-          }
-        }
-        publish();
-        find_bin(by_weight, target, base_cnt, base_w);
-        if (S.found_bin < 0) return kAll;   // (the range always holds the crossing)
-        base_cnt = S.found_cnt;
-        base_w = S.found_w;
-        in_cnt = S.found_in_cnt;
-        key_lo += uint32_t(S.found_bin) << shift;
-        key_hi = min(key_hi, key_lo + ((1u << shift) - 1));
-        __syncthreads();
-      }
-    };
-    // The first level's bin b holds the keys with floor(64 d) == b.
-    auto first_lo = [](int bin) { return __float_as_uint(float(bin) * (1.f / 64.f)); };
-
-    publish();               // the histograms are complete
-    u64 total_k = 0;
-    bool whole = true;       // top-k keeps every token with a weight
-    if (use_k) {
-      find_bin(false, u64(top_k), 0, 0);
-      const int bin = S.found_bin;
-      const u64 bc = S.found_cnt, bw = S.found_w, ic = S.found_in_cnt;
-      __syncthreads();
-      // the last bin holds only weights of 0: a cut inside it leaves the draw as it is
-      if (bin >= 0 && bin < kBins - 1) {
-        whole = false;
-        cut = refine(first_lo(bin), first_lo(bin + 1) - 1, false, u64(top_k), bc, bw, ic, total_k);
-        limit_id = cut;
-      }
-    }
-    if (use_p) {
-      if (whole) {
-        u64 t = warp_sum64(sum);
-        if (lane == 0) S.warp_a[warp] = t;
-        __syncthreads();
-        t = warp_sum64(S.warp_a[lane]);
-        if (tid < C) *cluster.map_shared_rank(&S.slot[0][rank], tid) = t;
-        publish();
-        for (int r = 0; r < C; ++r) total_k += S.slot[0][r];
-      }
-      const u64 target = max(share(total_k, top_p), u64(1));
-      if (dirty) {
-        publish();
-        for (int i = tid; i < kBins; i += kThreads) S.cnt[i] = S.wlo[i] = S.whi[i] = 0;
-        __syncthreads();
-        for (int i = s0 + lane; i < s1; i += 32) add_to_bin(bin_of(x[i]), weight(x[i]));
-        publish();
-      }
-      find_bin(true, target, 0, 0);
-      const int bin = S.found_bin;
-      const u64 bc = S.found_cnt, bw = S.found_w, ic = S.found_in_cnt;
-      __syncthreads();
-      if (bin >= 0) {
-        u64 unused;
-        cut = min(limit_id, refine(first_lo(bin), first_lo(bin + 1) - 1, true, target, bc, bw, ic, unused));
-      }
-    }
-    publish();               // shared slots may be reused
-  }
-
-  // ---------------------------------------------------------------- the draw
+  const bool filter = use_k || use_p;
   const uint32_t min_w = min_p > 0.f ? uint32_t(fminf(min_p, 1.f) * 2147483648.f) : 0u;
-  auto kept = [&](int i) -> uint32_t {
-    const float d = x[i];
-    const uint32_t w = weight(d);
-    const u64 id = (u64(__float_as_uint(d)) << 32) | uint32_t(lo + i);
-    return (id <= cut && w >= min_w) ? w : 0u;
+  const bool plain_t = temp == 1.f;
+  u64 sum = 0;                // of the weights; without a filter of the kept ones
+  for (int i = s0 + 2 * lane; i < s1; i += 64) {
+    float d[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float l = i + j < s1 ? x[i + j] : ninf;
+      d[j] = l == top ? 0.f : add_rn(top, -l);
+      if (!plain_t && l != top) d[j] = div_rn(d[j], temp);
+      d[j] = d[j] == d[j] ? fminf(d[j], 64.f) : 64.f;
+    }
+    const uint2 w = weight2(d[0], d[1]);
+    x[i] = d[0];
+    if (i + 1 < s1) x[i + 1] = d[1];
+    if (filter) {
+      sum += u64(w.x) + w.y;
+      const int b0 = bin_of(d[0]), b1 = bin_of(d[1]);
+      if (b0 < kNear) add_to_bin(b0, w.x);
+      if (b1 < kNear) add_to_bin(b1, w.y);    // (past the end: d = 64)
+    } else {
+      sum += u64(w.x >= min_w ? w.x : 0u) + (w.y >= min_w ? w.y : 0u);
+    }
+  }
+  auto publish = [&] { cluster.sync(); };
+  // this warp's, the lower CTAs' and the cluster's sum of `v`, one value a lane, through slot[which]
+  auto sum_over = [&](u64 v, int which, u64& mine, u64& below, u64& total) {
+    mine = warp_sum64(v);
+    if (lane == 0) S.warp_a[warp] = mine;
+    __syncthreads();
+    const u64 w = S.warp_a[lane];
+    if (warp == 0) {
+      const u64 t = warp_sum64(w);
+      if (lane < C) *cluster.map_shared_rank(&S.slot[which][rank], lane) = t;
+    }
+    publish();
+    below = warp_sum64(lane < warp ? w : 0);   // the lower warps of this CTA
+    total = 0;
+    for (int r = 0; r < C; ++r) {
+      if (r < rank) below += S.slot[which][r];
+      total += S.slot[which][r];
+    }
   };
-  sum = 0;
-  for (int i = s0 + lane; i < s1; i += 32) sum += kept(i);
-  sum = warp_sum64(sum);
-  __syncthreads();
-  if (lane == 0) S.warp_a[warp] = sum;
-  __syncthreads();
-  if (warp == 0) {
-    const u64 t = warp_sum64(S.warp_a[lane]);
-    if (lane < C) *cluster.map_shared_rank(&S.slot[0][rank], lane) = t;
-  }
-  cluster.sync();            // the last access to another CTA's shared memory is behind it
-  u64 total = 0, ahead = 0;
-  for (int r = 0; r < C; ++r) {
-    if (r < rank) ahead += S.slot[0][r];
-    total += S.slot[0][r];
-  }
-  const float u = a.u[b];
-  const u64 target = share(total, fminf(u, 0.99999994f));
-  for (int i = 0; i < warp; ++i) ahead += S.warp_a[i];
-  if (target >= ahead && target < ahead + sum) {
+  // The first token in vocabulary order whose inclusive cumulative kept weight exceeds the target.
+  auto draw = [&](auto kept, u64 mine, u64 below, u64 total) {
+    const u64 target = share(total, fminf(a.u[b], 0.99999994f));
+    if (target < below || target >= below + mine) return;
     for (int base = s0; base < s1; base += 32) {
       const int i = base + lane;
-      u64 inc = i < s1 ? kept(i) : 0u;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const u64 up = __shfl_up_sync(0xffffffffu, inc, d);
-        if (lane >= d) inc += up;
-      }
-      const uint32_t hit = __ballot_sync(0xffffffffu, ahead + inc > target);
+      const u64 inc = warp_scan64(i < s1 ? kept(i) : 0u, lane);
+      const uint32_t hit = __ballot_sync(0xffffffffu, below + inc > target);
       if (hit) {
         if (lane == __ffs(hit) - 1) a.token[b] = lo + i;
         break;
       }
-      ahead += __shfl_sync(0xffffffffu, inc, 31);
+      below += __shfl_sync(0xffffffffu, inc, 31);
+    }
+  };
+  u64 mine, below, total;
+  sum_over(sum, 0, mine, below, total);
+  auto kept_plain = [&](int i) {
+    const uint32_t w = weight(x[i]);
+    return w >= min_w ? w : 0u;
+  };
+  if (!filter) {
+    draw(kept_plain, mine, below, total);
+    return;
+  }
+
+  // ---------------------------------------------------------------- the bin of the cut
+  // Sums of two bins a thread over the cluster, then a block scan to the bin where the count (or the
+  // weight) reaches `target`.
+  auto find_bin = [&](bool by_weight, u64 target, u64 base_cnt, u64 base_w) {
+    u64 c[2] = {0, 0}, w[2] = {0, 0};
+    for (int r = 0; r < C; ++r) {
+      const uint4 h = reinterpret_cast<const uint4*>(cluster.map_shared_rank(&S.hist[0], r))[tid];
+      c[0] += h.x & 0xffffu;
+      w[0] += (u64(h.x >> 16) << 32) + h.y;
+      c[1] += h.z & 0xffffu;
+      w[1] += (u64(h.z >> 16) << 32) + h.w;
+    }
+    const u64 ic = warp_scan64(c[0] + c[1], lane), iw = warp_scan64(w[0] + w[1], lane);
+    if (tid == 0) S.found_bin = -1;
+    if (lane == 31) {
+      S.warp_a[warp] = ic;
+      S.warp_b[warp] = iw;
+    }
+    __syncthreads();
+    u64 ec = base_cnt + ic - c[0] - c[1] + warp_sum64(lane < warp ? S.warp_a[lane] : 0);
+    u64 ew = base_w + iw - w[0] - w[1] + warp_sum64(lane < warp ? S.warp_b[lane] : 0);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const u64 before = by_weight ? ew : ec, in = by_weight ? w[j] : c[j];
+      if (before < target && before + in >= target) {
+        S.found_bin = 2 * tid + j;
+        S.found_cnt = ec;
+        S.found_w = ew;
+        S.found_in_cnt = c[j];
+      }
+      ec += c[j];
+      ew += w[j];
+    }
+    __syncthreads();
+  };
+  auto fill_all = [&] {
+    publish();                 // every CTA has read the histogram in place
+    clear();
+    __syncthreads();
+    for (int i = s0 + lane; i < s1; i += 32) add_to_bin(bin_of(x[i]), weight(x[i]));
+    publish();
+  };
+  bool by_k = use_k;
+  u64 limit = by_k ? u64(top_k) : max(share(total, top_p), u64(1));
+  find_bin(!by_k, limit, 0, 0);
+  if (S.found_bin < 0) {
+    fill_all();
+    find_bin(!by_k, limit, 0, 0);
+    if (by_k && (S.found_bin < 0 || S.found_bin == kBins - 1)) {
+      // the last bin holds only weights of 0: a top-k cut inside it leaves the draw as it is
+      by_k = false;
+      if (use_p) {
+        limit = max(share(total, top_p), u64(1));
+        __syncthreads();
+        find_bin(true, limit, 0, 0);
+      }
     }
   }
+  const bool cut_somewhere = by_k || use_p;
+  const int bin = S.found_bin;
+  const u64 bin_cnt = S.found_cnt, bin_w = S.found_w, bin_in = S.found_in_cnt;
+  // the first level's bin b holds the keys of d in [b / 64, (b + 1) / 64)
+  auto first_lo = [](int i) { return __float_as_uint(float(i) * (1.f / 64.f)); };
+
+  // ---------------------------------------------------------------- few tokens up to it: one CTA's work
+  if (cut_somewhere && bin >= 0 && bin_cnt + bin_in <= kList) {
+    const float end = float(bin + 1) * (1.f / 64.f);
+    for (int i = s0 + lane; i < s1; i += 32) {
+      const float d = x[i];
+      if (d < end) S.list[atomicAdd(&S.list_n, 1)] = (u64(__float_as_uint(d)) << 32) | uint32_t(lo + i);
+    }
+    publish();
+    if (rank == 0) {
+      int n_all = 0;
+      for (int r = 0; r < C; ++r) {
+        const Shared* o = cluster.map_shared_rank(&S, r);
+        const int m = min(o->list_n, kList - n_all);
+        if (tid >= n_all && tid < n_all + m) S.all[tid] = o->list[tid - n_all];
+        n_all += m;
+      }
+      int size = 32;
+      while (size < n_all) size <<= 1;
+      u64 v = tid < n_all ? S.all[tid] : kAll;      // (its own element: no barrier needed)
+      v = sort64(v, size, S.list, tid);
+      const bool here = tid < n_all;
+      const uint32_t w = here ? weight(__uint_as_float(uint32_t(v >> 32))) : 0u;
+      auto scan = [&](u64 val, u64& inc, u64& all) {   // inclusive over the block
+        inc = warp_scan64(val, lane);
+        __syncthreads();
+        if (lane == 31) S.warp_a[warp] = inc;
+        __syncthreads();
+        const u64 o = S.warp_a[lane];
+        inc += warp_sum64(lane < warp ? o : 0);
+        all = warp_sum64(o);
+      };
+      u64 inc, all;
+      bool keep = here && (!by_k || tid < top_k);
+      scan(keep ? w : 0u, inc, all);
+      if (use_p) keep = keep && inc - w < (by_k ? max(share(all, top_p), u64(1)) : limit);
+      keep = keep && w >= min_w;
+      // kept tokens in vocabulary order, (index, weight)
+      v = sort64(keep ? (u64(uint32_t(v)) << 32) | w : kAll, size, S.list, tid);
+      keep = v != kAll;
+      scan(keep ? uint32_t(v) : 0u, inc, all);
+      const u64 target = share(all, fminf(a.u[b], 0.99999994f));
+      if (keep && inc > target && inc - uint32_t(v) <= target) a.token[b] = (long long)(v >> 32);
+    }
+    publish();                 // rank 0 has read the lists
+    return;
+  }
+
+  // ---------------------------------------------------------------- the general way
+  // The (key, index) of the last kept token, by key ranges: tokens in [key_lo, key_hi], `in_cnt` of
+  // them, `base` ahead of them. kept_w: the kept prefix's weight.
+  u64 cut = kAll;
+  const uint32_t* xkey = reinterpret_cast<const uint32_t*>(x);
+  bool dirty = false;          // the first level's histogram has been overwritten
+  auto order_list = [&](uint32_t key_lo, uint32_t key_hi, bool by_weight, u64 target, u64 base_cnt, u64 base_w, u64& kept_w) {
+    for (int i = s0 + lane; i < s1; i += 32) {
+      const uint32_t key = xkey[i];
+      if (key >= key_lo && key <= key_hi) {
+        const int at = atomicAdd(&S.list_n, 1);
+        if (at < kList) S.list[at] = (u64(key) << 32) | uint32_t(lo + i);
+      }
+    }
+    publish();
+    int n_all = 0;
+    for (int r = 0; r < C; ++r) {
+      const Shared* o = cluster.map_shared_rank(&S, r);
+      const int m = min(o->list_n, kList - n_all);
+      if (tid >= n_all && tid < n_all + m) S.all[tid] = o->list[tid - n_all];
+      n_all += m;
+    }
+    u64 v = tid < n_all ? S.all[tid] : kAll;
+    publish();                 // every CTA has read the lists
+    if (tid == 0) S.list_n = 0;
+    int size = 32;
+    while (size < n_all) size <<= 1;
+    v = sort64(v, size, S.list, tid);
+    const uint32_t w = tid < n_all ? weight(__uint_as_float(uint32_t(v >> 32))) : 0u;
+    u64 inc = warp_scan64(w, lane);
+    __syncthreads();
+    if (lane == 31) S.warp_a[warp] = inc;
+    if (tid == 0) {
+      S.found = kAll;
+      S.found_w = 0;
+    }
+    __syncthreads();
+    inc += base_w + warp_sum64(lane < warp ? S.warp_a[lane] : 0);
+    const u64 before = by_weight ? inc - w : base_cnt + tid, in = by_weight ? w : 1;
+    if (tid < n_all && before < target && before + in >= target) {
+      S.found = v;
+      S.found_w = inc;
+    }
+    __syncthreads();
+    kept_w = S.found_w;
+    const u64 id = S.found;
+    __syncthreads();
+    return id;
+  };
+  auto refine = [&](uint32_t key_lo, uint32_t key_hi, bool by_weight, u64 target, u64 base_cnt, u64 base_w, u64 in_cnt,
+                    u64& kept_w) -> u64 {
+    while (true) {
+      if (in_cnt <= kList) return order_list(key_lo, key_hi, by_weight, target, base_cnt, base_w, kept_w);
+      if (key_lo == key_hi) {
+        // more equal keys than the list holds: the m-th of them in index order is the last kept
+        const uint32_t w = weight(__uint_as_float(key_lo));
+        const u64 m = by_weight ? (target - base_w + w - 1) / max(w, 1u) : target - base_cnt;
+        kept_w = base_w + m * w;
+        u64 cnt = 0, warp_cnt, ahead, ties;
+        for (int i = s0 + lane; i < s1; i += 32) cnt += xkey[i] == key_lo;
+        sum_over(cnt, 1, warp_cnt, ahead, ties);
+        if (ahead < m && ahead + warp_cnt >= m) {
+          for (int base = s0; base < s1; base += 32) {
+            const int i = base + lane;
+            const uint32_t hit = __ballot_sync(0xffffffffu, i < s1 && xkey[i] == key_lo);
+            const int c = __popc(hit);
+            if (ahead + c >= m) {
+              const int nth = int(m - ahead);   // 1-based among the hits of these 32
+              if ((hit >> lane & 1) && __popc(hit & ((2u << lane) - 1)) == nth) {
+                const u64 id = (u64(key_lo) << 32) | uint32_t(lo + i);
+                for (int r = 0; r < C; ++r) *cluster.map_shared_rank(&S.found, r) = id;
+              }
+              break;
+            }
+            ahead += c;
+          }
+        }
+        publish();
+        const u64 id = S.found;
+        publish();
+        return id;
+      }
+      publish();               // every CTA has read the previous histogram
+      dirty = true;
+      clear();
+      __syncthreads();
+      int shift = 0;
+      while (((key_hi - key_lo) >> shift) >= kBins) ++shift;
+      for (int i = s0 + lane; i < s1; i += 32) {
+        const uint32_t key = xkey[i];
+        if (key >= key_lo && key <= key_hi) add_to_bin((key - key_lo) >> shift, weight(x[i]));
+      }
+      publish();
+      find_bin(by_weight, target, base_cnt, base_w);
+      if (S.found_bin < 0) return kAll;   // (the range always holds the crossing)
+      base_cnt = S.found_cnt;
+      base_w = S.found_w;
+      in_cnt = S.found_in_cnt;
+      key_lo += uint32_t(S.found_bin) << shift;
+      key_hi = min(key_hi, key_lo + ((1u << shift) - 1));
+      __syncthreads();
+    }
+  };
+  __syncthreads();
+  if (cut_somewhere && bin >= 0) {
+    u64 total_k;
+    cut = refine(first_lo(bin), first_lo(bin + 1) - 1, !by_k, limit, bin_cnt, bin_w, bin_in, total_k);
+    if (by_k && use_p) {
+      // top-p among the tokens that top-k kept
+      limit = max(share(total_k, top_p), u64(1));
+      if (dirty) fill_all();
+      find_bin(true, limit, 0, 0);
+      const int p_bin = S.found_bin;
+      const u64 p_cnt = S.found_cnt, p_w = S.found_w, p_in = S.found_in_cnt;
+      __syncthreads();
+      u64 unused;
+      if (p_bin >= 0) cut = min(cut, refine(first_lo(p_bin), first_lo(p_bin + 1) - 1, true, limit, p_cnt, p_w, p_in, unused));
+    }
+  }
+  const uint32_t cut_key = uint32_t(cut >> 32);
+  auto kept = [&](int i) -> uint32_t {
+    const float d = x[i];
+    const uint32_t key = __float_as_uint(d);
+    if (key > cut_key) return 0u;
+    const uint32_t w = weight(d);
+    return (((u64(key) << 32) | uint32_t(lo + i)) <= cut && w >= min_w) ? w : 0u;
+  };
+  sum = 0;
+  for (int i = s0 + lane; i < s1; i += 32) sum += kept(i);
+  __syncthreads();
+  publish();                   // slot[0] has been read everywhere
+  sum_over(sum, 0, mine, below, total);   // its barrier: the last access to another CTA's memory is behind it
+  draw(kept, mine, below, total);
 }
 
 template <bool BF16>

@@ -18,13 +18,15 @@
 // are read from memory once. A histogram over d (bins of 1/64; counts and weight sums of the tokens
 // near the maximum, of all of them only if the cut lies further out) gives the bin where the cut
 // falls; the tokens up to it, usually a few dozen, are gathered into one CTA, sorted and finished
-// there. More than 1024 of them (a large k, a flat row, ties) take the general way: histograms of the
+// there. More than 512 of them (a large k, a flat row, ties) take the general way: histograms of the
 // crossing bin until it is small, or the exact tie, then one pass over the kept tokens.
 // Bound: instructions per token (distance, weight) for many rows, the chain of cluster barriers for
 // one. The weight's polynomial runs on packed pairs.
 #include <cooperative_groups.h>
 
 #include <cuda_bf16.h>
+
+#include <algorithm>
 
 #include "common.cuh"
 #include "launch.h"
@@ -40,13 +42,14 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;        // two CTAs an SM: one row's barriers hide behind another's work
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
-constexpr int kList = 1024;         // tokens that are ordered directly (one a thread)
+constexpr int kList = kThreads;     // tokens that are ordered directly (one a thread)
 constexpr int kNear = 640;          // bins of the first histogram: d < 10
 constexpr int kMaxCluster = 16;     // 16 is the hardware's limit (above 8: opt-in)
 constexpr int kMaxSlice = 45056;    // floats of a row in one CTA's shared memory
+constexpr int kPairSlice = 20480;   // and where two CTAs share an SM
 constexpr u64 kAll = ~0ull;
 
 // The fixed operations of the weight: no contraction, no flush of subnormals, whatever the flags.
@@ -80,8 +83,10 @@ __device__ __forceinline__ uint2 weight2(float d0, float d1) {
   // w in (0.7, 1.42): 24 significant bits at 2^-23 or 2^-24 (one place further down)
   auto fixed = [](float v, float sum) {
     const uint32_t b = __float_as_uint(v);
-    const int sh = int(__float_as_uint(sum) & 0x7f) + int(127 - (b >> 23));
-    return sh > 31 ? 0u : ((b << 8) | 0x80000000u) >> sh;
+    const uint32_t sh = (__float_as_uint(sum) & 0x7f) + (127 - (b >> 23));
+    uint32_t r;
+    asm("shr.u32 %0, %1, %2;" : "=r"(r) : "r"((b << 8) | 0x80000000u), "r"(sh));   // (more than 31: 0)
+    return r;
   };
   return make_uint2(fixed(w.x, t.x), fixed(w.y, t.y));
 }
@@ -118,6 +123,7 @@ struct __align__(16) Shared {
   // this CTA's histogram: x: count in the low 16 bits, carries of y in the high ones; y: weights
   // modulo 2^32 (a slice has at most 45056 tokens of at most 2^31, so both halves hold)
   uint2 hist[kBins];
+  u64 slot_c[kMaxCluster], slot_w[kMaxCluster];  // totals of every CTA's segment of bins
   u64 list[kList];                               // this CTA's gathered tokens, (key, index)
   u64 all[kList];                                // the cluster's
   u64 warp_a[kWarps], warp_b[kWarps];
@@ -151,12 +157,15 @@ __device__ __forceinline__ u64 sort64(u64 v, int size, u64* buf, int tid) {
 }
 
 template <bool BF16>
-__global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a, int slice) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int slice) {
   extern __shared__ __align__(16) unsigned char raw[];
   Shared& S = *reinterpret_cast<Shared*>(raw);
-  float* x = reinterpret_cast<float*>(raw + sizeof(Shared));
   cg::cluster_group cluster = cg::this_cluster();
   const int C = int(cluster.num_blocks()), rank = int(cluster.block_rank());
+  // the cluster's sums of this CTA's segment of bins, and its slice of the row
+  u64* seg_w = reinterpret_cast<u64*>(raw + sizeof(Shared));
+  uint32_t* seg_c = reinterpret_cast<uint32_t*>(seg_w + kBins / C);
+  float* x = reinterpret_cast<float*>(seg_c + kBins / C);
   const int b = blockIdx.x / C;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_trigger();
@@ -173,30 +182,25 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a, int s
     const char* src = reinterpret_cast<const char*>(a.logits) + ((long)b * a.row_stride + lo) * esize;
     const bool aligned = reinterpret_cast<uintptr_t>(src) % 16 == 0;
     const int nv = aligned ? n / vec : 0;
-    for (int i = tid; i < nv; i += kThreads) {
+    float4* x4 = reinterpret_cast<float4*>(x);
+#pragma unroll 4
+    for (int i = tid; i < nv; i += kThreads) {   // (fmaxf passes NaN over)
       const uint4 v = ld_nc_v4(src + (long)i * 16);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (BF16) {
-          float f0 = bf16_lo(w[j]), f1 = bf16_hi(w[j]);
-          f0 = f0 == f0 ? f0 : ninf;
-          f1 = f1 == f1 ? f1 : ninf;
-          x[i * 8 + 2 * j] = f0;
-          x[i * 8 + 2 * j + 1] = f1;
-          top = fmaxf(top, fmaxf(f0, f1));
-        } else {
-          float f = __uint_as_float(w[j]);
-          f = f == f ? f : ninf;
-          x[i * 4 + j] = f;
-          top = fmaxf(top, f);
-        }
+      if (BF16) {
+        const float4 p = make_float4(bf16_lo(v.x), bf16_hi(v.x), bf16_lo(v.y), bf16_hi(v.y));
+        const float4 q = make_float4(bf16_lo(v.z), bf16_hi(v.z), bf16_lo(v.w), bf16_hi(v.w));
+        x4[2 * i] = p;
+        x4[2 * i + 1] = q;
+        top = fmaxf(top, fmaxf(fmaxf(fmaxf(p.x, p.y), fmaxf(p.z, p.w)), fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w))));
+      } else {
+        const float4 p = make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+        x4[i] = p;
+        top = fmaxf(top, fmaxf(fmaxf(p.x, p.y), fmaxf(p.z, p.w)));
       }
     }
     for (int i = nv * vec + tid; i < n; i += kThreads) {
-      float f = BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(src)[i])
-                     : reinterpret_cast<const float*>(src)[i];
-      f = f == f ? f : ninf;
+      const float f = BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(src)[i])
+                           : reinterpret_cast<const float*>(src)[i];
       x[i] = f;
       top = fmaxf(top, f);
     }
@@ -217,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a, int s
   float* wf = reinterpret_cast<float*>(S.warp_a);
   if (lane == 0) wf[warp] = top;
   cluster.sync();      // every CTA of the cluster runs: its shared memory may be written
-  top = warp_max(wf[lane]);
+  top = warp_max(wf[lane % kWarps]);
   if (tid < C) *cluster.map_shared_rank(&S.fslot[rank], tid) = top;
   cluster.sync();
   top = S.fslot[0];
@@ -260,25 +264,35 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a, int s
   };
   const bool filter = use_k || use_p;
   const uint32_t min_w = min_p > 0.f ? uint32_t(fminf(min_p, 1.f) * 2147483648.f) : 0u;
-  const bool plain_t = temp == 1.f;
+  // (top - l) / T, correctly rounded: by the reciprocal and one correction of the quotient (Markstein
+  // 1990: with r = RN(1 / T), q = RN(x r) and e = x - q T exact in a fused multiply-add, RN(q + e r)
+  // is RN(x / T)) where no step can leave the normal range (a finite top of at least 2^-30 keeps every
+  // nonzero difference above 2^-60); else by division. fminf(NaN, 64) = 64: NaN logits and
+  // infinite distances end beyond every weight.
+  const float inv_t = div_rn(1.f, temp);
+  const bool by_inverse = temp >= 0x1p-60f && temp <= 0x1p60f && fabsf(top) >= 0x1p-30f && fabsf(top) < 3.4e38f;
+  auto distance2 = [&](float2 l) {
+    if (by_inverse) {
+      const float2 v = __fadd2_rn(make_float2(top, top), make_float2(-l.x, -l.y));
+      const float2 r = make_float2(inv_t, inv_t), q = __fmul2_rn(v, r);
+      const float2 e = __ffma2_rn(make_float2(-q.x, -q.y), make_float2(temp, temp), v);
+      const float2 d = __ffma2_rn(e, r, q);
+      return make_float2(fminf(d.x, 64.f), fminf(d.y, 64.f));
+    }
+    auto one = [&](float v) { return v == top ? 0.f : fminf(div_rn(add_rn(top, -v), temp), 64.f); };
+    return make_float2(one(l.x), one(l.y));
+  };
   u64 sum = 0;                // of the weights; without a filter of the kept ones
   for (int i = s0 + 2 * lane; i < s1; i += 64) {
-    float d[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const float l = i + j < s1 ? x[i + j] : ninf;
-      d[j] = l == top ? 0.f : add_rn(top, -l);
-      if (!plain_t && l != top) d[j] = div_rn(d[j], temp);
-      d[j] = d[j] == d[j] ? fminf(d[j], 64.f) : 64.f;
-    }
-    const uint2 w = weight2(d[0], d[1]);
-    x[i] = d[0];
-    if (i + 1 < s1) x[i + 1] = d[1];
+    // (slices start 8 elements aligned and a pair past the end stays inside the slice's memory)
+    float2 d = distance2(*reinterpret_cast<const float2*>(x + i));
+    if (i + 1 >= s1) d.y = 64.f;
+    const uint2 w = weight2(d.x, d.y);
+    *reinterpret_cast<float2*>(x + i) = d;
     if (filter) {
       sum += u64(w.x) + w.y;
-      const int b0 = bin_of(d[0]), b1 = bin_of(d[1]);
-      if (b0 < kNear) add_to_bin(b0, w.x);
-      if (b1 < kNear) add_to_bin(b1, w.y);    // (past the end: d = 64)
+      if (d.x < kNear / 64.f) add_to_bin(bin_of(d.x), w.x);
+      if (d.y < kNear / 64.f) add_to_bin(bin_of(d.y), w.y);
     } else {
       sum += u64(w.x >= min_w ? w.x : 0u) + (w.y >= min_w ? w.y : 0u);
     }
@@ -289,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a, int s
     mine = warp_sum64(v);
     if (lane == 0) S.warp_a[warp] = mine;
     __syncthreads();
-    const u64 w = S.warp_a[lane];
+    const u64 w = lane < kWarps ? S.warp_a[lane] : 0;
     if (warp == 0) {
       const u64 t = warp_sum64(w);
       if (lane < C) *cluster.map_shared_rank(&S.slot[which][rank], lane) = t;
@@ -329,39 +343,76 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a, int s
   }
 
   // ---------------------------------------------------------------- the bin of the cut
-  // Sums of two bins a thread over the cluster, then a block scan to the bin where the count (or the
-  // weight) reaches `target`.
-  auto find_bin = [&](bool by_weight, u64 target, u64 base_cnt, u64 base_w) {
-    u64 c[2] = {0, 0}, w[2] = {0, 0};
-    for (int r = 0; r < C; ++r) {
-      const uint4 h = reinterpret_cast<const uint4*>(cluster.map_shared_rank(&S.hist[0], r))[tid];
-      c[0] += h.x & 0xffffu;
-      w[0] += (u64(h.x >> 16) << 32) + h.y;
-      c[1] += h.z & 0xffffu;
-      w[1] += (u64(h.z >> 16) << 32) + h.w;
+  // The bin of the first `bins` where the cluster's count (or weight) reaches `target`. Every CTA sums
+  // one segment of the bins over the cluster (reading all of every histogram in every CTA would take
+  // C times the distributed-memory traffic, which is what this costs), the segments' totals say whose
+  // segment the crossing is in, and that CTA tells the others.
+  auto find_bin = [&](int bins, bool by_weight, u64 target, u64 base_cnt, u64 base_w) {
+    const int per = bins / C;                  // C is a power of two of at most 16, bins 640 or 2048
+    const int from = tid % C;
+    for (int p = tid; p < bins; p += kThreads) {           // (bins and threads are multiples of 32)
+      const int i = p / C;
+      const uint2 h = *cluster.map_shared_rank(&S.hist[rank * per + i], from);
+      u64 c = h.x & 0xffffu, w = (u64(h.x >> 16) << 32) + h.y;
+      for (int o = C >> 1; o > 0; o >>= 1) {
+        c += __shfl_xor_sync(0xffffffffu, c, o);
+        w += __shfl_xor_sync(0xffffffffu, w, o);
+      }
+      if (from == 0) {
+        seg_c[i] = uint32_t(c);
+        seg_w[i] = w;
+      }
     }
-    const u64 ic = warp_scan64(c[0] + c[1], lane), iw = warp_scan64(w[0] + w[1], lane);
-    if (tid == 0) S.found_bin = -1;
+    __syncthreads();
+    const int mine_n = (per + kThreads - 1) / kThreads;    // bins a thread looks at
+    u64 tc = 0, tw = 0;
+    for (int j = 0; j < mine_n; ++j) {
+      const int i = tid * mine_n + j;
+      if (i < per) {
+        tc += seg_c[i];
+        tw += seg_w[i];
+      }
+    }
+    const u64 ic = warp_scan64(tc, lane), iw = warp_scan64(tw, lane);
     if (lane == 31) {
       S.warp_a[warp] = ic;
       S.warp_b[warp] = iw;
     }
+    if (tid == 0) S.found_bin = -1;
     __syncthreads();
-    u64 ec = base_cnt + ic - c[0] - c[1] + warp_sum64(lane < warp ? S.warp_a[lane] : 0);
-    u64 ew = base_w + iw - w[0] - w[1] + warp_sum64(lane < warp ? S.warp_b[lane] : 0);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const u64 before = by_weight ? ew : ec, in = by_weight ? w[j] : c[j];
-      if (before < target && before + in >= target) {
-        S.found_bin = 2 * tid + j;
-        S.found_cnt = ec;
-        S.found_w = ew;
-        S.found_in_cnt = c[j];
+    const u64 oc = lane < kWarps ? S.warp_a[lane] : 0, ow = lane < kWarps ? S.warp_b[lane] : 0;
+    if (warp == 0) {
+      const u64 t0 = warp_sum64(oc), t1 = warp_sum64(ow);
+      if (lane < C) {
+        *cluster.map_shared_rank(&S.slot_c[rank], lane) = t0;
+        *cluster.map_shared_rank(&S.slot_w[rank], lane) = t1;
       }
-      ec += c[j];
-      ew += w[j];
     }
-    __syncthreads();
+    publish();
+    u64 ec = base_cnt + ic - tc + warp_sum64(lane < warp ? oc : 0);
+    u64 ew = base_w + iw - tw + warp_sum64(lane < warp ? ow : 0);
+    for (int r = 0; r < rank; ++r) {
+      ec += S.slot_c[r];
+      ew += S.slot_w[r];
+    }
+    for (int j = 0; j < mine_n; ++j) {
+      const int i = tid * mine_n + j;
+      if (i >= per) break;
+      const u64 c = seg_c[i], w = seg_w[i];
+      const u64 before = by_weight ? ew : ec, in = by_weight ? w : c;
+      if (before < target && before + in >= target) {
+        for (int r = 0; r < C; ++r) {
+          Shared* o = cluster.map_shared_rank(&S, r);
+          o->found_bin = rank * per + i;
+          o->found_cnt = ec;
+          o->found_w = ew;
+          o->found_in_cnt = c;
+        }
+      }
+      ec += c;
+      ew += w;
+    }
+    publish();
   };
   auto fill_all = [&] {
     publish();                 // every CTA has read the histogram in place
@@ -372,17 +423,17 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a, int s
   };
   bool by_k = use_k;
   u64 limit = by_k ? u64(top_k) : max(share(total, top_p), u64(1));
-  find_bin(!by_k, limit, 0, 0);
+  find_bin(kNear, !by_k, limit, 0, 0);
   if (S.found_bin < 0) {
     fill_all();
-    find_bin(!by_k, limit, 0, 0);
+    find_bin(kBins, !by_k, limit, 0, 0);
     if (by_k && (S.found_bin < 0 || S.found_bin == kBins - 1)) {
       // the last bin holds only weights of 0: a top-k cut inside it leaves the draw as it is
       by_k = false;
       if (use_p) {
         limit = max(share(total, top_p), u64(1));
-        __syncthreads();
-        find_bin(true, limit, 0, 0);
+        publish();             // found_bin has been read everywhere
+        find_bin(kBins, true, limit, 0, 0);
       }
     }
   }
@@ -395,9 +446,10 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a, int s
   // ---------------------------------------------------------------- few tokens up to it: one CTA's work
   if (cut_somewhere && bin >= 0 && bin_cnt + bin_in <= kList) {
     const float end = float(bin + 1) * (1.f / 64.f);
-    for (int i = s0 + lane; i < s1; i += 32) {
-      const float d = x[i];
-      if (d < end) S.list[atomicAdd(&S.list_n, 1)] = (u64(__float_as_uint(d)) << 32) | uint32_t(lo + i);
+    for (int i = s0 + 2 * lane; i < s1; i += 64) {
+      const float2 d = *reinterpret_cast<const float2*>(x + i);   // (past the end: 64)
+      if (d.x < end) S.list[atomicAdd(&S.list_n, 1)] = (u64(__float_as_uint(d.x)) << 32) | uint32_t(lo + i);
+      if (d.y < end) S.list[atomicAdd(&S.list_n, 1)] = (u64(__float_as_uint(d.y)) << 32) | uint32_t(lo + i + 1);
     }
     publish();
     if (rank == 0) {
@@ -419,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a, int s
         __syncthreads();
         if (lane == 31) S.warp_a[warp] = inc;
         __syncthreads();
-        const u64 o = S.warp_a[lane];
+        const u64 o = lane < kWarps ? S.warp_a[lane] : 0;
         inc += warp_sum64(lane < warp ? o : 0);
         all = warp_sum64(o);
       };
@@ -532,14 +584,13 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a, int s
         if (key >= key_lo && key <= key_hi) add_to_bin((key - key_lo) >> shift, weight(x[i]));
       }
       publish();
-      find_bin(by_weight, target, base_cnt, base_w);
+      find_bin(kBins, by_weight, target, base_cnt, base_w);
       if (S.found_bin < 0) return kAll;   // (the range always holds the crossing)
       base_cnt = S.found_cnt;
       base_w = S.found_w;
       in_cnt = S.found_in_cnt;
       key_lo += uint32_t(S.found_bin) << shift;
       key_hi = min(key_hi, key_lo + ((1u << shift) - 1));
-      __syncthreads();
     }
   };
   __syncthreads();
@@ -550,7 +601,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a, int s
       // top-p among the tokens that top-k kept
       limit = max(share(total_k, top_p), u64(1));
       if (dirty) fill_all();
-      find_bin(true, limit, 0, 0);
+      else publish();
+      find_bin(kBins, true, limit, 0, 0);
       const int p_bin = S.found_bin;
       const u64 p_cnt = S.found_cnt, p_w = S.found_w, p_in = S.found_in_cnt;
       __syncthreads();
@@ -576,11 +628,12 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a, int s
 
 template <bool BF16>
 cudaError_t launch(const SampleArgs& a, int cluster, int slice, cudaStream_t s) {
-  const size_t smem = sizeof(Shared) + size_t(slice) * sizeof(float);
+  auto bytes = [](int c, int n) { return sizeof(Shared) + size_t(kBins / c) * 12 + size_t(n) * sizeof(float); };
+  const size_t smem = bytes(cluster, slice);
   auto kernel = sample_kernel<BF16>;
   cudaError_t e = once_per_device_kernel(reinterpret_cast<const void*>(kernel), [&] {
     cudaError_t r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         int(sizeof(Shared) + kMaxSlice * sizeof(float)));
+                                         int(std::max(bytes(8, kMaxSlice), bytes(1, kPairSlice))));
     if (r == cudaSuccess) r = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     return r;
   });
@@ -609,10 +662,12 @@ const char* sample(const SampleArgs& a, cudaStream_t s) {
   if (a.V < 1) return "sample: no tokens";
   if (a.V > kMaxCluster * kMaxSlice) return "sample: at most 720896 tokens a row";
   if ((long)a.B * kMaxCluster > 0x7fffffffl) return "sample: too many rows";
-  // CTAs a row: enough to hold it, and more while there are SMs without a row
+  // CTAs a row: enough that two of them fit an SM (16 are the limit: longer slices beyond), and more
+  // while there are SMs without a row. 128256 tokens: 8 CTAs for many rows, 16 for a few.
   int cluster = 1;
-  while (cluster * kMaxSlice < a.V) cluster *= 2;
-  while (cluster < 8 && 2l * cluster * a.B <= a.num_sms && a.V / (2 * cluster) >= 2048) cluster *= 2;
+  while (cluster < 8 && cluster * kPairSlice < a.V) cluster *= 2;   // (one CTA: 20480 tokens at most)
+  while (cluster < kMaxCluster && cluster * kMaxSlice < a.V) cluster *= 2;
+  while (cluster < kMaxCluster && 2l * cluster * a.B <= a.num_sms && a.V / (2 * cluster) >= 2048) cluster *= 2;
   const int slice = ((a.V + cluster - 1) / cluster + 7) / 8 * 8;
   const cudaError_t e = a.bf16 ? launch<true>(a, cluster, slice, s) : launch<false>(a, cluster, slice, s);
   return e == cudaSuccess ? nullptr : cudaGetErrorString(e);

@@ -15,10 +15,9 @@
 // are 0; u has 24 bits and cannot reach them.
 //
 // One cluster per row: each CTA holds a contiguous slice of the row in shared memory, so the logits
-// are read from memory once. A histogram over d (bins of 1/64; counts and weight sums of the tokens
-// near the maximum, of all of them only if the cut lies further out) gives the bin where the cut
-// falls; the tokens up to it, usually a few dozen, are gathered into one CTA, sorted and finished
-// there. More than 512 of them (a large k, a flat row, ties) take the general way: histograms of the
+// are read from memory once. A histogram over d (bins of 1/64; counts for top-k, counts
+// and weight sums for top-p) gives the bin where the cut falls; the tokens up to it, usually a few
+// dozen, are sent to one CTA, sorted and finished there. More than 512 of them (a large k, a flat row, ties) take the general way: histograms of the
 // crossing bin until it is small, or the exact tie, then one pass over the kept tokens.
 // Bound: instructions per token (distance, weight) for many rows, the chain of cluster barriers for
 // one. The weight's polynomial runs on packed pairs.
@@ -46,7 +45,6 @@ constexpr int kThreads = 512;        // two CTAs an SM: one row's barriers hide 
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kList = kThreads;     // tokens that are ordered directly (one a thread)
-constexpr int kNear = 640;          // bins of the first histogram: d < 10
 constexpr int kMaxCluster = 16;     // 16 is the hardware's limit (above 8: opt-in)
 constexpr int kMaxSlice = 45056;    // floats of a row in one CTA's shared memory
 constexpr int kPairSlice = 20480;   // and where two CTAs share an SM
@@ -168,6 +166,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
   float* x = reinterpret_cast<float*>(seg_c + kBins / C);
   const int b = blockIdx.x / C;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  cluster.barrier_arrive();   // waited for before the first access to another CTA's shared memory
   pdl_trigger();
   pdl_wait();
 
@@ -220,7 +219,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
   top = warp_max(top);
   float* wf = reinterpret_cast<float*>(S.warp_a);
   if (lane == 0) wf[warp] = top;
-  cluster.sync();      // every CTA of the cluster runs: its shared memory may be written
+  cluster.barrier_wait();
+  __syncthreads();
   top = warp_max(wf[lane % kWarps]);
   if (tid < C) *cluster.map_shared_rank(&S.fslot[rank], tid) = top;
   cluster.sync();
@@ -282,17 +282,22 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     auto one = [&](float v) { return v == top ? 0.f : fminf(div_rn(add_rn(top, -v), temp), 64.f); };
     return make_float2(one(l.x), one(l.y));
   };
-  u64 sum = 0;                // of the weights; without a filter of the kept ones
+  u64 sum = 0;                // without a filter: of the kept weights
   for (int i = s0 + 2 * lane; i < s1; i += 64) {
     // (slices start 8 elements aligned and a pair past the end stays inside the slice's memory)
     float2 d = distance2(*reinterpret_cast<const float2*>(x + i));
-    if (i + 1 >= s1) d.y = 64.f;
-    const uint2 w = weight2(d.x, d.y);
+    const bool two = i + 1 < s1;
+    if (!two) d.y = 64.f;
     *reinterpret_cast<float2*>(x + i) = d;
-    if (filter) {
-      sum += u64(w.x) + w.y;
-      if (d.x < kNear / 64.f) add_to_bin(bin_of(d.x), w.x);
-      if (d.y < kNear / 64.f) add_to_bin(bin_of(d.y), w.y);
+    if (use_k) {              // counts alone
+      atomicAdd(&S.hist[bin_of(d.x)].x, 1u);
+      if (two) atomicAdd(&S.hist[bin_of(d.y)].x, 1u);
+      continue;
+    }
+    const uint2 w = weight2(d.x, d.y);
+    if (use_p) {
+      add_to_bin(bin_of(d.x), w.x);
+      if (two) add_to_bin(bin_of(d.y), w.y);
     } else {
       sum += u64(w.x >= min_w ? w.x : 0u) + (w.y >= min_w ? w.y : 0u);
     }
@@ -316,41 +321,53 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
       total += S.slot[which][r];
     }
   };
-  // The first token in vocabulary order whose inclusive cumulative kept weight exceeds the target.
+  // The first token in vocabulary order whose inclusive cumulative kept weight exceeds the target. The
+  // warp whose run holds it looks at 1024 tokens at a time: each lane sums 32 neighbours (starting at
+  // its own offset among them, for the banks), then the lanes share the 32 of the lane that reaches it.
   auto draw = [&](auto kept, u64 mine, u64 below, u64 total) {
     const u64 target = share(total, fminf(a.u[b], 0.99999994f));
     if (target < below || target >= below + mine) return;
-    for (int base = s0; base < s1; base += 32) {
-      const int i = base + lane;
-      const u64 inc = warp_scan64(i < s1 ? kept(i) : 0u, lane);
+    for (int base = s0; base < s1; base += 1024) {
+      u64 v = 0;
+      for (int j = 0; j < 32; ++j) {
+        const int i = base + 32 * lane + ((j + lane) & 31);
+        v += i < s1 ? kept(i) : 0u;
+      }
+      const u64 inc = warp_scan64(v, lane);
       const uint32_t hit = __ballot_sync(0xffffffffu, below + inc > target);
       if (hit) {
-        if (lane == __ffs(hit) - 1) a.token[b] = lo + i;
+        const int l = __ffs(hit) - 1;
+        below += __shfl_sync(0xffffffffu, inc - v, l);
+        const int i = base + 32 * l + lane;
+        const u64 one = warp_scan64(i < s1 ? kept(i) : 0u, lane);
+        const uint32_t at = __ballot_sync(0xffffffffu, below + one > target);
+        if (lane == __ffs(at) - 1) a.token[b] = lo + i;
         break;
       }
       below += __shfl_sync(0xffffffffu, inc, 31);
     }
   };
   u64 mine, below, total;
-  sum_over(sum, 0, mine, below, total);
-  auto kept_plain = [&](int i) {
-    const uint32_t w = weight(x[i]);
-    return w >= min_w ? w : 0u;
-  };
   if (!filter) {
-    draw(kept_plain, mine, below, total);
+    sum_over(sum, 0, mine, below, total);
+    draw([&](int i) {
+      const uint32_t w = weight(x[i]);
+      return w >= min_w ? w : 0u;
+    }, mine, below, total);
     return;
   }
 
   // ---------------------------------------------------------------- the bin of the cut
-  // The bin of the first `bins` where the cluster's count (or weight) reaches `target`. Every CTA sums
+  // The bin where the cluster's count (or weight) reaches `target` (or top_p of the weight in all the
+  // bins, for target 0, which it returns). Every CTA sums
   // one segment of the bins over the cluster (reading all of every histogram in every CTA would take
   // C times the distributed-memory traffic, which is what this costs), the segments' totals say whose
   // segment the crossing is in, and that CTA tells the others.
-  auto find_bin = [&](int bins, bool by_weight, u64 target, u64 base_cnt, u64 base_w) {
-    const int per = bins / C;                  // C is a power of two of at most 16, bins 640 or 2048
+  auto find_bin = [&](bool by_weight, u64 target, u64 base_cnt, u64 base_w) {
+    const int per = kBins / C;                 // C is a power of two of at most 16
     const int from = tid % C;
-    for (int p = tid; p < bins; p += kThreads) {           // (bins and threads are multiples of 32)
+#pragma unroll
+    for (int p = tid; p < kBins; p += kThreads) {
       const int i = p / C;
       const uint2 h = *cluster.map_shared_rank(&S.hist[rank * per + i], from);
       u64 c = h.x & 0xffffu, w = (u64(h.x >> 16) << 32) + h.y;
@@ -391,10 +408,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     publish();
     u64 ec = base_cnt + ic - tc + warp_sum64(lane < warp ? oc : 0);
     u64 ew = base_w + iw - tw + warp_sum64(lane < warp ? ow : 0);
-    for (int r = 0; r < rank; ++r) {
-      ec += S.slot_c[r];
-      ew += S.slot_w[r];
+    u64 all_w = 0;
+    for (int r = 0; r < C; ++r) {
+      if (r < rank) {
+        ec += S.slot_c[r];
+        ew += S.slot_w[r];
+      }
+      all_w += S.slot_w[r];
     }
+    if (target == 0) target = max(share(all_w, top_p), u64(1));
     for (int j = 0; j < mine_n; ++j) {
       const int i = tid * mine_n + j;
       if (i >= per) break;
@@ -413,6 +435,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
       ew += w;
     }
     publish();
+    return target;
   };
   auto fill_all = [&] {
     publish();                 // every CTA has read the histogram in place
@@ -422,47 +445,40 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     publish();
   };
   bool by_k = use_k;
-  u64 limit = by_k ? u64(top_k) : max(share(total, top_p), u64(1));
-  find_bin(kNear, !by_k, limit, 0, 0);
-  if (S.found_bin < 0) {
-    fill_all();
-    find_bin(kBins, !by_k, limit, 0, 0);
-    if (by_k && (S.found_bin < 0 || S.found_bin == kBins - 1)) {
-      // the last bin holds only weights of 0: a top-k cut inside it leaves the draw as it is
-      by_k = false;
-      if (use_p) {
-        limit = max(share(total, top_p), u64(1));
-        publish();             // found_bin has been read everywhere
-        find_bin(kBins, true, limit, 0, 0);
-      }
+  publish();                   // the histograms are complete
+  u64 limit = find_bin(!by_k, by_k ? u64(top_k) : 0, 0, 0);
+  if (by_k && (S.found_bin < 0 || S.found_bin == kBins - 1)) {
+    // the last bin holds only weights of 0: a top-k cut inside it leaves the draw as it is
+    by_k = false;
+    if (use_p) {
+      fill_all();
+      limit = find_bin(true, 0, 0, 0);
     }
   }
   const bool cut_somewhere = by_k || use_p;
-  const int bin = S.found_bin;
-  const u64 bin_cnt = S.found_cnt, bin_w = S.found_w, bin_in = S.found_in_cnt;
+  int bin = S.found_bin;
+  u64 bin_cnt = S.found_cnt, bin_w = S.found_w, bin_in = S.found_in_cnt;
   // the first level's bin b holds the keys of d in [b / 64, (b + 1) / 64)
   auto first_lo = [](int i) { return __float_as_uint(float(i) * (1.f / 64.f)); };
 
   // ---------------------------------------------------------------- few tokens up to it: one CTA's work
   if (cut_somewhere && bin >= 0 && bin_cnt + bin_in <= kList) {
     const float end = float(bin + 1) * (1.f / 64.f);
+    Shared* to = cluster.map_shared_rank(&S, 0);
+    auto send = [&](float d, int i) {
+      if (d < end) to->all[atomicAdd(&to->list_n, 1)] = (u64(__float_as_uint(d)) << 32) | uint32_t(lo + i);
+    };
     for (int i = s0 + 2 * lane; i < s1; i += 64) {
       const float2 d = *reinterpret_cast<const float2*>(x + i);   // (past the end: 64)
-      if (d.x < end) S.list[atomicAdd(&S.list_n, 1)] = (u64(__float_as_uint(d.x)) << 32) | uint32_t(lo + i);
-      if (d.y < end) S.list[atomicAdd(&S.list_n, 1)] = (u64(__float_as_uint(d.y)) << 32) | uint32_t(lo + i + 1);
+      send(d.x, i);
+      send(d.y, i + 1);
     }
-    publish();
+    publish();                 // the last access to another CTA's shared memory is behind it
     if (rank == 0) {
-      int n_all = 0;
-      for (int r = 0; r < C; ++r) {
-        const Shared* o = cluster.map_shared_rank(&S, r);
-        const int m = min(o->list_n, kList - n_all);
-        if (tid >= n_all && tid < n_all + m) S.all[tid] = o->list[tid - n_all];
-        n_all += m;
-      }
+      const int n_all = S.list_n;
       int size = 32;
       while (size < n_all) size <<= 1;
-      u64 v = tid < n_all ? S.all[tid] : kAll;      // (its own element: no barrier needed)
+      u64 v = tid < n_all ? S.all[tid] : kAll;
       v = sort64(v, size, S.list, tid);
       const bool here = tid < n_all;
       const uint32_t w = here ? weight(__uint_as_float(uint32_t(v >> 32))) : 0u;
@@ -487,7 +503,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
       const u64 target = share(all, fminf(a.u[b], 0.99999994f));
       if (keep && inc > target && inc - uint32_t(v) <= target) a.token[b] = (long long)(v >> 32);
     }
-    publish();                 // rank 0 has read the lists
     return;
   }
 
@@ -506,14 +521,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
       }
     }
     publish();
-    int n_all = 0;
+    // lane r looks at CTA r's list; thread t takes token t of the lists laid end to end
+    int len = lane < C ? min(cluster.map_shared_rank(&S, lane)->list_n, kList) : 0, n_all = 0;
+    u64 v = kAll;
     for (int r = 0; r < C; ++r) {
-      const Shared* o = cluster.map_shared_rank(&S, r);
-      const int m = min(o->list_n, kList - n_all);
-      if (tid >= n_all && tid < n_all + m) S.all[tid] = o->list[tid - n_all];
+      const int m = __shfl_sync(0xffffffffu, len, r);
+      if (tid >= n_all && tid < n_all + m) v = cluster.map_shared_rank(&S, r)->list[tid - n_all];
       n_all += m;
     }
-    u64 v = tid < n_all ? S.all[tid] : kAll;
     publish();                 // every CTA has read the lists
     if (tid == 0) S.list_n = 0;
     int size = 32;
@@ -584,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
         if (key >= key_lo && key <= key_hi) add_to_bin((key - key_lo) >> shift, weight(x[i]));
       }
       publish();
-      find_bin(kBins, by_weight, target, base_cnt, base_w);
+      find_bin(by_weight, target, base_cnt, base_w);
       if (S.found_bin < 0) return kAll;   // (the range always holds the crossing)
       base_cnt = S.found_cnt;
       base_w = S.found_w;
@@ -594,6 +609,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     }
   };
   __syncthreads();
+  if (by_k && use_p) {         // top-p needs the kept weight: sums beside the counts
+    fill_all();
+    find_bin(false, limit, 0, 0);
+    bin = S.found_bin;
+    bin_cnt = S.found_cnt;
+    bin_w = S.found_w;
+    bin_in = S.found_in_cnt;
+    __syncthreads();
+  }
   if (cut_somewhere && bin >= 0) {
     u64 total_k;
     cut = refine(first_lo(bin), first_lo(bin + 1) - 1, !by_k, limit, bin_cnt, bin_w, bin_in, total_k);
@@ -602,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
       limit = max(share(total_k, top_p), u64(1));
       if (dirty) fill_all();
       else publish();
-      find_bin(kBins, true, limit, 0, 0);
+      find_bin(true, limit, 0, 0);
       const int p_bin = S.found_bin;
       const u64 p_cnt = S.found_cnt, p_w = S.found_w, p_in = S.found_in_cnt;
       __syncthreads();

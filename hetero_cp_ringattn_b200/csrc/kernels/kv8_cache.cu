@@ -73,94 +73,184 @@ __device__ __forceinline__ void rope_q(const AppendArgs& a, long item) {
   }
 }
 
-// One warp per (unit, KV head, k or v): the maximum over the unit's tokens, the scale, the codes.
+// A unit's place: checked before anything is addressed by it.
+struct UnitAt {
+  int t0, n, p0, start;   // first token, tokens, first position, first offset in the block
+  int page;               // -1: nothing to do
+};
+
+__device__ __forceinline__ UnitAt unit_at(const AppendArgs& a, long ui, bool report) {
+  UnitAt z{0, 0, 0, 0, -1};
+  if (ui >= a.U) return z;
+  const int4 u = a.unit[ui];
+  if (u.x < 0) return z;
+  const int P = a.c.P, block = u.w / P;
+  z.t0 = u.y;
+  z.n = u.z;
+  z.p0 = u.w;
+  z.start = u.w - block * P;
+  const bool ok = u.x < a.R && u.y >= 0 && u.z >= 1 && u.z <= a.T - u.y && u.w >= 0 && z.start + u.z <= P && block < a.width;
+  const int page = ok ? a.table[(long)u.x * a.width + block] : -1;
+  if (page >= 0 && page < a.c.pages) z.page = page;
+  else if (report) report_error(a.status, int(StatusCode::kOutOfBounds), 402, page, int(ui));
+  return z;
+}
+
+// 16 values of one (token, chunk): k rotated, v as it is.
+template <int DT, int D>
+__device__ __forceinline__ void unit_values(const AppendArgs& a, int t, int pos, int col, bool rotate, int chunk, float (&x1)[8],
+                                            float (&x2)[8]) {
+  const long at = (long)t * a.row_stride + (long)col * D + chunk * 8;
+  load8<DT>(a.x, at, x1);
+  load8<DT>(a.x, at + D / 2, x2);
+  if (rotate) {
+    float c[8], s[8];
+    load_cos_sin(a, min(pos, a.max_pos - 1), chunk * 8, c, s);
+    rotate8(x1, x2, c, s);
+  }
+}
+
+__device__ __forceinline__ float max_abs(const float (&x1)[8], const float (&x2)[8], float m) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = fmaxf(m, fmaxf(fabsf(x1[j]), fabsf(x2[j])));
+  return m;
+}
+
+// 16 stored codes times f (a block whose scale has grown).
+template <bool INT8>
+__device__ __forceinline__ void rescale16(uint8_t* at, float f) {
+  uint4* p = reinterpret_cast<uint4*>(at);
+  const uint4 v = *p;
+  const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+  uint32_t out[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t lo, hi;
+    decode4<INT8>(in[j], lo, hi);
+    const float2 x = half2_floats(lo), y = half2_floats(hi);
+    out[j] = encode4<INT8>(x.x * f, x.y * f, y.x * f, y.y * f);
+  }
+  *p = make_uint4(out[0], out[1], out[2], out[3]);
+}
+
+template <int D, bool INT8>
+__device__ __forceinline__ void store_codes(uint8_t* row, int chunk, const float (&x1)[8], const float (&x2)[8], float inv) {
+  uint2* p = reinterpret_cast<uint2*>(row + chunk * 8);
+  p[0] = make_uint2(encode4<INT8>(x1[0] * inv, x1[1] * inv, x1[2] * inv, x1[3] * inv),
+                    encode4<INT8>(x1[4] * inv, x1[5] * inv, x1[6] * inv, x1[7] * inv));
+  p[D / 16] = make_uint2(encode4<INT8>(x2[0] * inv, x2[1] * inv, x2[2] * inv, x2[3] * inv),
+                         encode4<INT8>(x2[4] * inv, x2[5] * inv, x2[6] * inv, x2[7] * inv));
+}
+
+__device__ __forceinline__ float* scale_at(const AppendArgs& a, int kv, int page, int h) {
+  return (kv ? a.c.v_scale : a.c.k_scale) + (long)page * a.c.scale_page_stride + (long)h * a.c.scale_head_stride;
+}
+
+__device__ __forceinline__ uint8_t* block_at(const AppendArgs& a, int kv, int page, int h) {
+  return (kv ? a.c.v : a.c.k) + (long)page * a.c.page_stride + (long)h * a.c.head_stride;
+}
+
+// Short units (a decode step): one warp per (unit, KV head, k or v). The first tokens' values stay in
+// registers between the maximum and the codes, later ones are read twice.
 template <int DT, int D, bool INT8>
-__device__ __forceinline__ void store_unit(const AppendArgs& a, long w) {
+__device__ __forceinline__ void store_short(const AppendArgs& a, long w) {
   constexpr int kChunks = D / 16, kTok = 32 / kChunks;  // tokens a warp covers at a time
   const int lane = threadIdx.x & 31;
   const int kv = int(w & 1);
   const long rest = w >> 1;
   const int h = int(rest % a.c.Hkv);
-  const long ui = rest / a.c.Hkv;
-  if (ui >= a.U) return;
-  const int4 u = a.unit[ui];
-  const int row = u.x, t0 = u.y, n = u.z, p0 = u.w;
-  if (row < 0) return;
-  const int P = a.c.P;
-  const int block = p0 / P, start = p0 - block * P;
-  const bool ok = row < a.R && t0 >= 0 && n >= 1 && t0 + n <= a.T && p0 >= 0 && start + n <= P && block < a.width;
-  const int page = ok ? a.table[(long)row * a.width + block] : -1;
-  if (page < 0 || page >= a.c.pages) {
-    if (lane == 0) report_error(a.status, int(StatusCode::kOutOfBounds), 402, page, int(ui));
-    return;
-  }
+  const UnitAt z = unit_at(a, rest / a.c.Hkv, lane == 0);
+  if (z.page < 0) return;
   const int chunk = lane % kChunks, sub = lane / kChunks;
   const int col = a.H + (kv ? a.c.Hkv : 0) + h;
-  auto row_values = [&](int i, float (&x1)[8], float (&x2)[8]) {
-    const long at = (long)(t0 + i) * a.row_stride + (long)col * D + chunk * 8;
-    load8<DT>(a.x, at, x1);
-    load8<DT>(a.x, at + D / 2, x2);
-    if (!kv) {
-      float c[8], s[8];
-      load_cos_sin(a, min(p0 + i, a.max_pos - 1), chunk * 8, c, s);
-      rotate8(x1, x2, c, s);
-    }
-  };
+  float* sc = scale_at(a, kv, z.page, h);
+  const float old = z.start > 0 ? *sc : 0.f;
+  float f1[8], f2[8], x1[8], x2[8];
   float amax = 0.f;
-  for (int i = sub; i < n; i += kTok) {
-    float x1[8], x2[8];
-    row_values(i, x1, x2);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fmaxf(fabsf(x1[j]), fabsf(x2[j])));
+  if (sub < z.n) {
+    unit_values<DT, D>(a, z.t0 + sub, z.p0 + sub, col, !kv, chunk, f1, f2);
+    amax = max_abs(f1, f2, amax);
+  }
+  for (int i = sub + kTok; i < z.n; i += kTok) {
+    unit_values<DT, D>(a, z.t0 + i, z.p0 + i, col, !kv, chunk, x1, x2);
+    amax = max_abs(x1, x2, amax);
   }
   amax = warp_max(amax);
-  float* scale_at = (kv ? a.c.v_scale : a.c.k_scale) + (long)page * a.c.scale_page_stride + (long)h * a.c.scale_head_stride;
-  const float old = start > 0 ? *scale_at : 0.f;
   const float scale = fmaxf(old, block_scale<INT8>(amax));
-  __syncwarp();
-  uint8_t* data = (kv ? a.c.v : a.c.k) + (long)page * a.c.page_stride + (long)h * a.c.head_stride;
-  if (start > 0 && scale > old) {
-    const float f = __fdiv_rn(old, scale);
-    for (int i = sub; i < start; i += kTok) {
-      uint4* p = reinterpret_cast<uint4*>(data + (long)i * a.c.token_stride + chunk * 16);
-      const uint4 v = *p;
-      uint32_t in[4] = {v.x, v.y, v.z, v.w}, out[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t lo, hi;
-        decode4<INT8>(in[j], lo, hi);
-        const float2 x = half2_floats(lo), y = half2_floats(hi);
-        out[j] = encode4<INT8>(x.x * f, x.y * f, y.x * f, y.y * f);
-      }
-      *p = make_uint4(out[0], out[1], out[2], out[3]);
-    }
-  }
-  if (lane == 0) *scale_at = scale;
+  uint8_t* data = block_at(a, kv, z.page, h);
+  if (z.start > 0 && scale > old)
+    for (int i = sub; i < z.start; i += kTok) rescale16<INT8>(data + (long)i * a.c.token_stride + chunk * 16, __fdiv_rn(old, scale));
+  if (lane == 0) *sc = scale;
   const float inv = __fdiv_rn(1.f, scale);  // exact: a power of two (an old scale may be another value)
-  for (int i = sub; i < n; i += kTok) {
-    float x1[8], x2[8];
-    row_values(i, x1, x2);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x1[j] *= inv;
-      x2[j] *= inv;
-    }
-    uint8_t* p = data + (long)(start + i) * a.c.token_stride + chunk * 8;
-    *reinterpret_cast<uint2*>(p) = make_uint2(encode4<INT8>(x1[0], x1[1], x1[2], x1[3]),
-                                              encode4<INT8>(x1[4], x1[5], x1[6], x1[7]));
-    *reinterpret_cast<uint2*>(p + D / 2) = make_uint2(encode4<INT8>(x2[0], x2[1], x2[2], x2[3]),
-                                                      encode4<INT8>(x2[4], x2[5], x2[6], x2[7]));
+  data += (long)z.start * a.c.token_stride;
+  if (sub < z.n) store_codes<D, INT8>(data + (long)sub * a.c.token_stride, chunk, f1, f2, inv);
+  for (int i = sub + kTok; i < z.n; i += kTok) {
+    unit_values<DT, D>(a, z.t0 + i, z.p0 + i, col, !kv, chunk, x1, x2);
+    store_codes<D, INT8>(data + (long)i * a.c.token_stride, chunk, x1, x2, inv);
   }
 }
 
+// Whole blocks (prompts): P D / 64 threads (at least a warp) per (unit, KV head, k or v), 64 values a
+// thread held in registers between the maximum and the codes: one pass over the input.
+constexpr int kItems = 4;
+
+__host__ __device__ constexpr int block_threads(int P, int D) { return P * D / 64 < 32 ? 32 : P * D / 64; }
+
 template <int DT, int D, bool INT8>
-__global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a, int q_ctas) {
+__device__ __forceinline__ void store_block(const AppendArgs& a, long cta) {
+  constexpr int kChunks = D / 16;
+  __shared__ float top[kThreads / 32];
+  const int team = block_threads(a.c.P, D);     // 32 to 256
+  const long w = cta * (kThreads / team) + threadIdx.x / team;
+  const int me = threadIdx.x % team;
+  const int kv = int(w & 1);
+  const long rest = w >> 1;
+  const int h = int(rest % a.c.Hkv);
+  const UnitAt z = unit_at(a, rest / a.c.Hkv, me == 0);
+  const bool some = z.page >= 0;
+  const int col = a.H + (kv ? a.c.Hkv : 0) + h;
+  float* sc = some ? scale_at(a, kv, z.page, h) : nullptr;
+  const float old = some && z.start > 0 ? *sc : 0.f;
+  float x1[kItems][8], x2[kItems][8];
+  float amax = 0.f;
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const int item = k * team + me, i = item / kChunks, chunk = item % kChunks;
+    if (some && i < z.n) unit_values<DT, D>(a, z.t0 + i, z.p0 + i, col, !kv, chunk, x1[k], x2[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < kItems; ++k)
+    if (some && (k * team + me) / kChunks < z.n) amax = max_abs(x1[k], x2[k], amax);
+  amax = warp_max(amax);
+  if ((threadIdx.x & 31) == 0) top[threadIdx.x / 32] = amax;
+  __syncthreads();              // (also: the old scale has been read before it is replaced)
+  if (!some) return;
+  const int first = (threadIdx.x / team) * (team / 32);
+  for (int i = 0; i < team / 32; ++i) amax = fmaxf(amax, top[first + i]);
+  const float scale = fmaxf(old, block_scale<INT8>(amax));
+  uint8_t* data = block_at(a, kv, z.page, h);
+  if (z.start > 0 && scale > old)
+    for (int item = me; item < z.start * kChunks; item += team)
+      rescale16<INT8>(data + (long)(item / kChunks) * a.c.token_stride + item % kChunks * 16, __fdiv_rn(old, scale));
+  if (me == 0) *sc = scale;
+  const float inv = __fdiv_rn(1.f, scale);
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const int item = k * team + me, i = item / kChunks;
+    if (i < z.n) store_codes<D, INT8>(data + (long)(z.start + i) * a.c.token_stride, item % kChunks, x1[k], x2[k], inv);
+  }
+}
+
+template <int DT, int D, bool INT8, bool SHORT>
+__global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a, int store_ctas) {
   pdl_trigger();
   pdl_wait();
-  if (int(blockIdx.x) < q_ctas) {
-    rope_q<DT, D>(a, (long)blockIdx.x * kThreads + threadIdx.x);
+  if (int(blockIdx.x) >= store_ctas) {
+    rope_q<DT, D>(a, ((long)blockIdx.x - store_ctas) * kThreads + threadIdx.x);
+  } else if (SHORT) {
+    store_short<DT, D, INT8>(a, (long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5));
   } else {
-    store_unit<DT, D, INT8>(a, ((long)blockIdx.x - q_ctas) * (kThreads / 32) + (threadIdx.x >> 5));
+    store_block<DT, D, INT8>(a, blockIdx.x);
   }
 }
 
@@ -168,10 +258,14 @@ template <int DT, int D, bool INT8>
 cudaError_t launch_append(const AppendArgs& a, cudaStream_t s) {
   const long items = (long)a.T * (D / 16) * ((a.H + kQHeads - 1) / kQHeads);
   const long q_ctas = (items + kThreads - 1) / kThreads;
-  const long warps = (long)a.U * a.c.Hkv * 2;
-  const long s_ctas = (warps + kThreads / 32 - 1) / (kThreads / 32);
+  // units of 4 tokens or more on average: whole blocks
+  const bool few = (long)a.T < 4l * a.U;
+  const long teams = (long)a.U * a.c.Hkv * 2, per = few ? kThreads / 32 : kThreads / block_threads(a.c.P, D);
+  const long s_ctas = (teams + per - 1) / per;
   if (q_ctas + s_ctas > 0x7fffffffl) return cudaErrorInvalidValue;
-  return launch_pdl(append_kernel<DT, D, INT8>, dim3(unsigned(q_ctas + s_ctas)), dim3(kThreads), 0, s, a, int(q_ctas));
+  const dim3 grid(unsigned(q_ctas + s_ctas)), block(kThreads);
+  return few ? launch_pdl(append_kernel<DT, D, INT8, true>, grid, block, 0, s, a, int(s_ctas))
+             : launch_pdl(append_kernel<DT, D, INT8, false>, grid, block, 0, s, a, int(s_ctas));
 }
 
 template <int DT, int D>

@@ -38,6 +38,7 @@ struct PlanArgs {
   int* ring;             // [ring_size] free pages, FIFO between the two counters
   const long long* counters;  // [2] head, tail
   int R, width, P, ring_size, max_tokens, max_units;
+  int shift;             // set by the launcher: log2 of a power-of-two P
   int* cu;               // [R + 1]
   int* row;              // [max_tokens]
   int* pos;              // [max_tokens]

@@ -6,12 +6,12 @@
 // and a "unit" per block that the new tokens touch, the work list of the append. A step that does
 // not fit (tokens, table width or free pages) changes nothing and says so in info[3].
 //
-// Bound: latency. The arrays are a few bytes per row and token, so one cluster of up to 8 CTAs
-// does the whole step in one launch: every CTA scans all rows (four sums at once), the cluster
-// barrier separates the reads of the state from its update (the new lengths and counters may
-// overwrite the old ones), and the CTAs share the tokens, units and pages to write. New pages are
-// looked up by their place in the ring rather than through the table, so no CTA depends on an
-// entry that another one writes.
+// Bound: latency. The arrays are a few bytes per row and token, so one launch does the whole step:
+// every CTA scans all rows (four sums at once) and the CTAs share the tokens, units and pages to
+// write. New pages are looked up by their place in the ring rather than through the table, so no CTA
+// depends on an entry that another one writes. Where the new lengths or counters overwrite the old
+// ones, the CTAs form one cluster (of at most 8) whose barrier separates the reads of the state from
+// its update; otherwise there are as many CTAs as the writes are worth.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -50,6 +50,14 @@ __device__ __forceinline__ int find_row(const int* off, int n, int x) {
   return lo;
 }
 
+// x mod n for x >= 0, in 32 bits where they hold it.
+__device__ __forceinline__ int modulo(long long x, int n) {
+  x = x < 0 ? 0 : x;
+  return (x >> 32) == 0 ? int(uint32_t(x) % uint32_t(n)) : int(x % n);
+}
+
+// SHIFT: the page size is 1 << a.shift. CLUSTER: the new state may overwrite the old one.
+template <bool SHIFT, bool CLUSTER>
 __global__ void __launch_bounds__(1024) plan_kernel(PlanArgs a) {
   extern __shared__ int sm[];
   int* s_cu = sm;                      // [R + 1] first token of each row
@@ -58,12 +66,13 @@ __global__ void __launch_bounds__(1024) plan_kernel(PlanArgs a) {
   int* s_back = s_need + a.R + 1;      // [R + 1] first page given back
   int* s_old = s_back + a.R + 1;       // [R]
   __shared__ Sums warp_tot[32];
-  cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, nth = blockDim.x, lane = tid & 31, warp = tid >> 5;
   pdl_trigger();
   pdl_wait();
 
   const int P = a.P;
+  auto pages_before = [&](int x) { return SHIFT ? x >> a.shift : x / P; };      // whole pages below position x
+  auto pages_for = [&](int x) { return SHIFT ? (x + P - 1) >> a.shift : (x + P - 1) / P; };
   const long long cap = (long long)a.width * P;
   const int per = (a.R + nth - 1) / nth;
   const int r0 = min(a.R, tid * per), r1 = min(a.R, r0 + per);
@@ -73,7 +82,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(PlanArgs a) {
   auto row_of = [&](int r, int& old) {
     const int add = a.add[r];
     old = int(min((long long)max(a.kv_len[r], 0), cap));
-    const int have = (old + P - 1) / P;
+    const int have = pages_for(old);
     Sums v{0, 0, 0, 0};
     if (add < 0) {
       v.back = have;
@@ -82,8 +91,8 @@ __global__ void __launch_bounds__(1024) plan_kernel(PlanArgs a) {
       if (end > cap) {
         wide = true;
       } else {
-        v.need = int((end + P - 1) / P) - have;
-        v.units = int((end + P - 1) / P) - old / P;
+        v.need = pages_for(int(end)) - have;
+        v.units = pages_for(int(end)) - pages_before(old);
       }
       v.n = add;
     }
@@ -102,11 +111,17 @@ __global__ void __launch_bounds__(1024) plan_kernel(PlanArgs a) {
   }
   if (lane == 31) warp_tot[warp] = inc;
   const bool any_wide = __syncthreads_or(wide);
-  Sums before{0, 0, 0, 0}, total{0, 0, 0, 0};
-  for (int w = 0; w < nth / 32; ++w) {
-    if (w == warp) before = total;
-    total = total + warp_tot[w];
+  Sums total = lane < nth / 32 ? warp_tot[lane] : Sums{0, 0, 0, 0};
+  const Sums own_warp = total;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const Sums up = shfl_up(total, d);
+    if (lane >= d) total = total + up;
   }
+  Sums before{__shfl_sync(0xffffffffu, total.n - own_warp.n, warp), __shfl_sync(0xffffffffu, total.units - own_warp.units, warp),
+              __shfl_sync(0xffffffffu, total.need - own_warp.need, warp), __shfl_sync(0xffffffffu, total.back - own_warp.back, warp)};
+  total = Sums{__shfl_sync(0xffffffffu, total.n, 31), __shfl_sync(0xffffffffu, total.units, 31),
+               __shfl_sync(0xffffffffu, total.need, 31), __shfl_sync(0xffffffffu, total.back, 31)};
   Sums ex{before.n + inc.n - own.n, before.units + inc.units - own.units, before.need + inc.need - own.need,
           before.back + inc.back - own.back};
   const long long avail = min(max(tail - head, 0ll), (long long)a.ring_size);
@@ -132,14 +147,15 @@ __global__ void __launch_bounds__(1024) plan_kernel(PlanArgs a) {
     s_need[a.R] = total.need;
     s_back[a.R] = total.back;
   }
-  // the state has been read by every CTA of the cluster: it may be overwritten from here on
-  cluster.sync();
+  // the state has been read by every CTA that will: it may be overwritten from here on
+  if (CLUSTER) cg::this_cluster().sync();
+  else __syncthreads();
 
   const int T = int(total.n), U = total.units;
-  const int crank = int(cluster.block_rank()), csize = int(cluster.num_blocks());
+  const int crank = blockIdx.x, csize = gridDim.x;
   const int gtid = crank * nth + tid, gn = csize * nth;
   const long long size = a.ring_size;
-  const int head_at = int(((head % size) + size) % size), tail_at = int(((tail % size) + size) % size);
+  const int head_at = modulo(head, a.ring_size), tail_at = modulo(tail, a.ring_size);
   // page i of those taken in this step: first the ring's, then the ones given back in this step
   auto taken = [&](int i) {
     if (i < avail) {
@@ -151,7 +167,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(PlanArgs a) {
     return a.table[(long)r * a.width + (j - s_back[r])];
   };
   auto page_of = [&](int r, int block) {
-    const int have = (s_old[r] + P - 1) / P;
+    const int have = pages_for(s_old[r]);
     return block < have ? a.table[(long)r * a.width + block] : taken(s_need[r] + block - have);
   };
 
@@ -189,7 +205,8 @@ __global__ void __launch_bounds__(1024) plan_kernel(PlanArgs a) {
         const int p = s_old[r] + t - s_cu[r];
         row[j] = r;
         pos[j] = p;
-        slot[j] = (long long)page_of(r, p / P) * P + p % P;
+        const int block = pages_before(p);
+        slot[j] = (long long)page_of(r, block) * P + (p - block * P);
       }
     }
     if (t0 + 4 <= a.max_tokens) {
@@ -210,7 +227,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(PlanArgs a) {
     if (i < U) {
       const int r = find_row(s_unit, a.R + 1, i);
       const int old = s_old[r], end = old + s_cu[r + 1] - s_cu[r];
-      const int block = old / P + i - s_unit[r];
+      const int block = pages_before(old) + i - s_unit[r];
       const int p0 = max(block * P, old), p1 = min((block + 1) * P, end);
       u = make_int4(r, s_cu[r] + p0 - old, p1 - p0, p0);
     }
@@ -218,7 +235,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(PlanArgs a) {
   }
   for (int i = gtid; i < total.need; i += gn) {
     const int r = find_row(s_need, a.R + 1, i);
-    a.table[(long)r * a.width + (s_old[r] + P - 1) / P + i - s_need[r]] = taken(i);
+    a.table[(long)r * a.width + pages_for(s_old[r]) + i - s_need[r]] = taken(i);
   }
   for (int i = gtid; i < total.back; i += gn) {
     const int r = find_row(s_back, a.R + 1, i);
@@ -229,41 +246,60 @@ __global__ void __launch_bounds__(1024) plan_kernel(PlanArgs a) {
 
 }  // namespace
 
-const char* plan_step(const PlanArgs& a, cudaStream_t s) {
+namespace {
+
+template <bool SHIFT, bool CLUSTER>
+cudaError_t launch(const PlanArgs& a, int ctas, int threads, cudaStream_t s) {
+  auto kernel = plan_kernel<SHIFT, CLUSTER>;
+  cudaError_t e = once_per_device_kernel(reinterpret_cast<const void*>(kernel), [&] {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (5 * kPlanMaxRows + 8) * int(sizeof(int)));
+  });
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(ctas));
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = (size_t(a.R + 1) * 4 + a.R) * sizeof(int);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (CLUSTER) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = unsigned(ctas);
+    attr[n].val.clusterDim.y = 1;
+    attr[n++].val.clusterDim.z = 1;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = unsigned(n);
+  return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+}  // namespace
+
+const char* plan_step(const PlanArgs& args, cudaStream_t s) {
+  PlanArgs a = args;
   if (a.R < 1 || a.R > kPlanMaxRows) return "plan_step: 1 to 4096 rows";
   if (a.P < 1 || a.width < 1 || a.ring_size < 1) return "plan_step: empty table, ring or page";
-  if ((long long)a.R * a.width >= (1ll << 31) || (long long)a.width * a.P >= (1ll << 31))
+  if ((long long)a.R * a.width >= (1ll << 31) || (long long)a.width * a.P >= (1ll << 30))
     return "plan_step: table too large";
   if (a.max_tokens < 1 || a.max_units < 1) return "plan_step: max_tokens and max_units must be positive";
   // threads for the rows and the token quads of a small step; CTAs for the writes of a large one
   const int quads = (a.max_tokens + 3) / 4;
   const int work = quads > a.max_units ? quads : a.max_units;
   const int most = work > a.R ? work : a.R;
-  const int threads = most <= 128 ? 128 : most <= 256 ? 256 : most <= 512 ? 512 : 1024;
+  const int threads = most <= 128 ? 128 : most <= 256 ? 256 : 512;
+  const bool in_place = a.kv_len_out == a.kv_len || a.counters_out == a.counters;
   int ctas = 1;
-  while (ctas < 8 && ctas * threads < work) ctas *= 2;
-  const size_t smem = (size_t(a.R + 1) * 4 + a.R) * sizeof(int);
-  static std::atomic<unsigned long long> done{0};
-  cudaError_t e = once_per_device(done, [] {
-    return cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (5 * kPlanMaxRows + 8) * int(sizeof(int)));
-  });
-  if (e != cudaSuccess) return cudaGetErrorString(e);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = unsigned(ctas);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, plan_kernel, a);
+  while (ctas < (in_place ? 8 : 128) && ctas * threads < work) ctas *= 2;
+  const bool cluster = in_place && ctas > 1;
+  a.shift = 0;
+  while ((1 << a.shift) < a.P) ++a.shift;
+  const bool shift = (1 << a.shift) == a.P;
+  const cudaError_t e = shift ? (cluster ? launch<true, true>(a, ctas, threads, s) : launch<true, false>(a, ctas, threads, s))
+                              : (cluster ? launch<false, true>(a, ctas, threads, s) : launch<false, false>(a, ctas, threads, s));
   return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
 }
 

@@ -41,35 +41,45 @@ __device__ __forceinline__ void load_cos_sin(const AppendArgs& a, int pos, int j
   load8<kF32>(a.sin_t, at, s);
 }
 
-// q of one (token, 8-element chunk) for every head of a group.
-constexpr int kQHeads = 8;
+// q of one (token, 8-element chunk) for the heads of a group, whose loads are all in flight before the
+// first is used.
+constexpr int kQHeads = 4;
 
 template <int DT, int D>
-__device__ __forceinline__ void rope_q(const AppendArgs& a, long item) {
-  constexpr int kChunks = D / 16;
+__device__ __forceinline__ void rope_q(const AppendArgs& a, uint32_t item) {
+  constexpr int kChunks = D / 16, kAtOnce = DT == kF32 ? (kQHeads + 1) / 2 : kQHeads;
   const int chunk = int(item % kChunks);
-  const long rest = item / kChunks;
-  const int groups = (a.H + kQHeads - 1) / kQHeads;
+  const uint32_t rest = item / kChunks, groups = uint32_t(a.H + kQHeads - 1) / kQHeads;
   const int t = int(rest / groups), h0 = int(rest % groups) * kQHeads;
   if (t >= a.T) return;
   const int pos = a.pos[t];
-  float c[8], s[8];
   const bool ok = pos >= 0 && pos < a.max_pos;
   if (!ok && chunk == 0 && h0 == 0) report_error(a.status, int(StatusCode::kOutOfBounds), 401, pos, t);
-  load_cos_sin(a, ok ? pos : 0, chunk * 8, c, s);
-  const int h1 = min(a.H, h0 + kQHeads);
-#pragma unroll 4
-  for (int h = h0; h < h1; ++h) {
-    float x1[8], x2[8];
-    const long at = (long)t * a.row_stride + (long)h * D + chunk * 8;
-    load8<DT>(a.x, at, x1);
-    load8<DT>(a.x, at + D / 2, x2);
-    rotate8(x1, x2, c, s);
-    uint4* o = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.q_out) + ((long)t * a.H + h) * D + chunk * 8);
-    o[0] = make_uint4(pack16(a.q_dtype, x1[0], x1[1]), pack16(a.q_dtype, x1[2], x1[3]),
-                      pack16(a.q_dtype, x1[4], x1[5]), pack16(a.q_dtype, x1[6], x1[7]));
-    o[D / 16] = make_uint4(pack16(a.q_dtype, x2[0], x2[1]), pack16(a.q_dtype, x2[2], x2[3]),
-                           pack16(a.q_dtype, x2[4], x2[5]), pack16(a.q_dtype, x2[6], x2[7]));
+  float c[8], s[8];
+#pragma unroll
+  for (int g = 0; g < kQHeads; g += kAtOnce) {
+    Raw8<DT> r1[kAtOnce], r2[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const long at = (long)t * a.row_stride + (long)min(h0 + g + i, a.H - 1) * D + chunk * 8;
+      r1[i] = load_raw8<DT>(a.x, at);
+      r2[i] = load_raw8<DT>(a.x, at + D / 2);
+    }
+    if (g == 0) load_cos_sin(a, ok ? pos : 0, chunk * 8, c, s);
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int h = h0 + g + i;
+      if (h >= a.H) break;
+      float x1[8], x2[8];
+      floats8<DT>(r1[i], x1);
+      floats8<DT>(r2[i], x2);
+      rotate8(x1, x2, c, s);
+      uint4* o = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.q_out) + ((long)t * a.H + h) * D + chunk * 8);
+      o[0] = make_uint4(pack16(a.q_dtype, x1[0], x1[1]), pack16(a.q_dtype, x1[2], x1[3]),
+                        pack16(a.q_dtype, x1[4], x1[5]), pack16(a.q_dtype, x1[6], x1[7]));
+      o[D / 16] = make_uint4(pack16(a.q_dtype, x2[0], x2[1]), pack16(a.q_dtype, x2[2], x2[3]),
+                             pack16(a.q_dtype, x2[4], x2[5]), pack16(a.q_dtype, x2[6], x2[7]));
+    }
   }
 }
 
@@ -79,9 +89,9 @@ struct UnitAt {
   int page;               // -1: nothing to do
 };
 
-__device__ __forceinline__ UnitAt unit_at(const AppendArgs& a, long ui, bool report) {
+__device__ __forceinline__ UnitAt unit_at(const AppendArgs& a, uint32_t ui, bool report) {
   UnitAt z{0, 0, 0, 0, -1};
-  if (ui >= a.U) return z;
+  if (ui >= uint32_t(a.U)) return z;
   const int4 u = a.unit[ui];
   if (u.x < 0) return z;
   const int P = a.c.P, block = u.w / P;
@@ -153,13 +163,13 @@ __device__ __forceinline__ uint8_t* block_at(const AppendArgs& a, int kv, int pa
 // Short units (a decode step): one warp per (unit, KV head, k or v). The first tokens' values stay in
 // registers between the maximum and the codes, later ones are read twice.
 template <int DT, int D, bool INT8>
-__device__ __forceinline__ void store_short(const AppendArgs& a, long w) {
+__device__ __forceinline__ void store_short(const AppendArgs& a, uint32_t w) {
   constexpr int kChunks = D / 16, kTok = 32 / kChunks;  // tokens a warp covers at a time
   const int lane = threadIdx.x & 31;
   const int kv = int(w & 1);
-  const long rest = w >> 1;
-  const int h = int(rest % a.c.Hkv);
-  const UnitAt z = unit_at(a, rest / a.c.Hkv, lane == 0);
+  const uint32_t rest = w >> 1;
+  const int h = int(rest % uint32_t(a.c.Hkv));
+  const UnitAt z = unit_at(a, rest / uint32_t(a.c.Hkv), lane == 0);
   if (z.page < 0) return;
   const int chunk = lane % kChunks, sub = lane / kChunks;
   const int col = a.H + (kv ? a.c.Hkv : 0) + h;
@@ -190,82 +200,125 @@ __device__ __forceinline__ void store_short(const AppendArgs& a, long w) {
   }
 }
 
-// Whole blocks (prompts): P D / 64 threads (at least a warp) per (unit, KV head, k or v), 64 values a
-// thread held in registers between the maximum and the codes: one pass over the input.
-constexpr int kItems = 4;
+// Whole blocks (prompts): P D / 32 threads per (unit, group of KV heads, k or v), 32 values of a head a
+// thread held in registers between the maximum and the codes: one pass over the input. The next
+// head's loads are in flight while a head is coded, and k's cosines and sines are loaded once.
+constexpr int kItems = 2;
 
-__host__ __device__ constexpr int block_threads(int P, int D) { return P * D / 64 < 32 ? 32 : P * D / 64; }
+__host__ __device__ constexpr int block_threads(int P, int D) { return P * D / 32; }
 
 template <int DT, int D, bool INT8>
-__device__ __forceinline__ void store_block(const AppendArgs& a, long cta) {
+__device__ __forceinline__ void store_block(const AppendArgs& a, uint32_t cta, int heads) {
   constexpr int kChunks = D / 16;
-  __shared__ float top[kThreads / 32];
-  const int team = block_threads(a.c.P, D);     // 32 to 256
-  const long w = cta * (kThreads / team) + threadIdx.x / team;
+  __shared__ float top[2][16];
+  const int team = block_threads(a.c.P, D);     // 32 to 512
+  const uint32_t w = cta * uint32_t(int(blockDim.x) / team) + uint32_t(int(threadIdx.x) / team);
   const int me = threadIdx.x % team;
   const int kv = int(w & 1);
-  const long rest = w >> 1;
-  const int h = int(rest % a.c.Hkv);
-  const UnitAt z = unit_at(a, rest / a.c.Hkv, me == 0);
-  const bool some = z.page >= 0;
-  const int col = a.H + (kv ? a.c.Hkv : 0) + h;
-  float* sc = some ? scale_at(a, kv, z.page, h) : nullptr;
-  const float old = some && z.start > 0 ? *sc : 0.f;
-  float x1[kItems][8], x2[kItems][8];
-  float amax = 0.f;
+  const uint32_t rest = w >> 1, groups = uint32_t((a.c.Hkv + heads - 1) / heads);
+  const int h0 = int(rest % groups) * heads, h1 = min(a.c.Hkv, h0 + heads);
+  const UnitAt z = unit_at(a, rest / groups, me == 0);
+  const int n = z.page >= 0 ? z.n : 0;
+  const int col0 = a.H + (kv ? a.c.Hkv : 0);
+  Raw8<DT> r1[kItems], r2[kItems];
+  float c[kItems][8], s[kItems][8];
+  auto fetch = [&](int h) {
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      const int item = k * team + me, i = item / kChunks, chunk = item % kChunks;
+      if (i < n) {
+        const long at = (long)(z.t0 + i) * a.row_stride + (long)(col0 + h) * D + chunk * 8;
+        r1[k] = load_raw8<DT>(a.x, at);
+        r2[k] = load_raw8<DT>(a.x, at + D / 2);
+      }
+    }
+  };
+  fetch(h0);
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
     const int item = k * team + me, i = item / kChunks, chunk = item % kChunks;
-    if (some && i < z.n) unit_values<DT, D>(a, z.t0 + i, z.p0 + i, col, !kv, chunk, x1[k], x2[k]);
+    if (!kv && i < n) load_cos_sin(a, min(z.p0 + i, a.max_pos - 1), chunk * 8, c[k], s[k]);
   }
+  for (int h = h0; h < h0 + heads; ++h) {     // (every team of the CTA makes all turns: barriers)
+    const bool some = n > 0 && h < h1;
+    float* sc = some ? scale_at(a, kv, z.page, h) : nullptr;
+    const float old = some && z.start > 0 ? *sc : 0.f;
+    float x1[kItems][8], x2[kItems][8];
+    float amax = 0.f;
 #pragma unroll
-  for (int k = 0; k < kItems; ++k)
-    if (some && (k * team + me) / kChunks < z.n) amax = max_abs(x1[k], x2[k], amax);
-  amax = warp_max(amax);
-  if ((threadIdx.x & 31) == 0) top[threadIdx.x / 32] = amax;
-  __syncthreads();              // (also: the old scale has been read before it is replaced)
-  if (!some) return;
-  const int first = (threadIdx.x / team) * (team / 32);
-  for (int i = 0; i < team / 32; ++i) amax = fmaxf(amax, top[first + i]);
-  const float scale = fmaxf(old, block_scale<INT8>(amax));
-  uint8_t* data = block_at(a, kv, z.page, h);
-  if (z.start > 0 && scale > old)
-    for (int item = me; item < z.start * kChunks; item += team)
-      rescale16<INT8>(data + (long)(item / kChunks) * a.c.token_stride + item % kChunks * 16, __fdiv_rn(old, scale));
-  if (me == 0) *sc = scale;
-  const float inv = __fdiv_rn(1.f, scale);
+    for (int k = 0; k < kItems; ++k)
+      if (some && (k * team + me) / kChunks < n) {
+        floats8<DT>(r1[k], x1[k]);
+        floats8<DT>(r2[k], x2[k]);
+        if (!kv) rotate8(x1[k], x2[k], c[k], s[k]);
+        amax = max_abs(x1[k], x2[k], amax);
+      }
+    if (h + 1 < h1) fetch(h + 1);
+    amax = warp_max(amax);
+    float* slot = top[h & 1];                 // (a slot is written again two barriers later)
+    if ((threadIdx.x & 31) == 0) slot[threadIdx.x / 32] = amax;
+    __syncthreads();                          // (also: the old scale has been read before it is replaced)
+    if (!some) continue;
+    const int first = (threadIdx.x / team) * (team / 32);
+    for (int i = 0; i < team / 32; ++i) amax = fmaxf(amax, slot[first + i]);
+    const float scale = fmaxf(old, block_scale<INT8>(amax));
+    uint8_t* data = block_at(a, kv, z.page, h);
+    if (z.start > 0 && scale > old)
+      for (int item = me; item < z.start * kChunks; item += team)
+        rescale16<INT8>(data + (long)(item / kChunks) * a.c.token_stride + item % kChunks * 16, __fdiv_rn(old, scale));
+    if (me == 0) *sc = scale;
+    const float inv = __fdiv_rn(1.f, scale);
 #pragma unroll
-  for (int k = 0; k < kItems; ++k) {
-    const int item = k * team + me, i = item / kChunks;
-    if (i < z.n) store_codes<D, INT8>(data + (long)(z.start + i) * a.c.token_stride, item % kChunks, x1[k], x2[k], inv);
+    for (int k = 0; k < kItems; ++k) {
+      const int item = k * team + me, i = item / kChunks;
+      if (i < n) store_codes<D, INT8>(data + (long)(z.start + i) * a.c.token_stride, item % kChunks, x1[k], x2[k], inv);
+    }
   }
 }
 
-template <int DT, int D, bool INT8, bool SHORT>
-__global__ void __launch_bounds__(kThreads) append_kernel(AppendArgs a, int store_ctas) {
+// Short units: one launch, the first CTAs store k and v, the others rotate q.
+template <int DT, int D, bool INT8>
+__global__ void __launch_bounds__(kThreads, 4) append_short_kernel(AppendArgs a, int store_ctas) {
   pdl_trigger();
   pdl_wait();
-  if (int(blockIdx.x) >= store_ctas) {
-    rope_q<DT, D>(a, ((long)blockIdx.x - store_ctas) * kThreads + threadIdx.x);
-  } else if (SHORT) {
-    store_short<DT, D, INT8>(a, (long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5));
-  } else {
-    store_block<DT, D, INT8>(a, blockIdx.x);
-  }
+  if (int(blockIdx.x) < store_ctas) store_short<DT, D, INT8>(a, blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5));
+  else rope_q<DT, D>(a, (blockIdx.x - store_ctas) * kThreads + threadIdx.x);
+}
+
+// Prompts: two launches, since the two want different shapes: k and v 128 registers a thread for what
+// they hold and prefetch, q as many threads as there are.
+template <int DT, int D, bool INT8>
+__global__ void __launch_bounds__(512, 1) append_block_kernel(AppendArgs a, int heads) {
+  pdl_trigger();
+  pdl_wait();
+  store_block<DT, D, INT8>(a, blockIdx.x, heads);
+}
+
+template <int DT, int D>
+__global__ void __launch_bounds__(kThreads, 4) rope_q_kernel(AppendArgs a) {
+  pdl_trigger();
+  pdl_wait();
+  rope_q<DT, D>(a, blockIdx.x * kThreads + threadIdx.x);
 }
 
 template <int DT, int D, bool INT8>
 cudaError_t launch_append(const AppendArgs& a, cudaStream_t s) {
   const long items = (long)a.T * (D / 16) * ((a.H + kQHeads - 1) / kQHeads);
   const long q_ctas = (items + kThreads - 1) / kThreads;
+  if (items + kThreads > 0x7fffffffl || (long)a.U * 2 * a.c.Hkv > 0x3fffffffl) return cudaErrorInvalidValue;
   // units of 4 tokens or more on average: whole blocks
-  const bool few = (long)a.T < 4l * a.U;
-  const long teams = (long)a.U * a.c.Hkv * 2, per = few ? kThreads / 32 : kThreads / block_threads(a.c.P, D);
-  const long s_ctas = (teams + per - 1) / per;
-  if (q_ctas + s_ctas > 0x7fffffffl) return cudaErrorInvalidValue;
-  const dim3 grid(unsigned(q_ctas + s_ctas)), block(kThreads);
-  return few ? launch_pdl(append_kernel<DT, D, INT8, true>, grid, block, 0, s, a, int(s_ctas))
-             : launch_pdl(append_kernel<DT, D, INT8, false>, grid, block, 0, s, a, int(s_ctas));
+  if ((long)a.T < 4l * a.U || a.U == 0) {
+    const long warps = (long)a.U * 2 * a.c.Hkv, s_ctas = (warps + kThreads / 32 - 1) / (kThreads / 32);
+    return launch_pdl(append_short_kernel<DT, D, INT8>, dim3(unsigned(q_ctas + s_ctas)), dim3(kThreads), 0, s, a, int(s_ctas));
+  }
+  const int team = block_threads(a.c.P, D), threads = team > 256 ? team : 256, per = threads / team;
+  // heads a team goes through: as many as leave four CTAs an SM
+  int heads = 1;
+  while (heads < a.c.Hkv && (long)a.U * 2 * (a.c.Hkv / (2 * heads)) >= 4l * 148 * per) heads *= 2;
+  const long teams = (long)a.U * 2 * ((a.c.Hkv + heads - 1) / heads);
+  cudaError_t e = launch_pdl(append_block_kernel<DT, D, INT8>, dim3(unsigned((teams + per - 1) / per)), dim3(threads), 0, s, a, heads);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(rope_q_kernel<DT, D>, dim3(unsigned(q_ctas)), dim3(kThreads), 0, s, a);
 }
 
 template <int DT, int D>
@@ -333,7 +386,7 @@ const char* check_cache(const Cache& c) {
 
 const char* rope_append(const AppendArgs& a, cudaStream_t s) {
   if (const char* e = check_cache(a.c)) return e;
-  if (a.T < 1 || a.U < 1) return nullptr;
+  if (a.T < 1) return nullptr;
   if (a.row_stride % 8 || reinterpret_cast<uintptr_t>(a.x) % 16 || reinterpret_cast<uintptr_t>(a.q_out) % 16)
     return "rope_append_kv8: rows must start on 16-byte boundaries";
   cudaError_t e = a.dtype == kF32 ? append_dim<kF32>(a, s) : a.dtype == kBF16 ? append_dim<kBF16>(a, s) : append_dim<kF16>(a, s);

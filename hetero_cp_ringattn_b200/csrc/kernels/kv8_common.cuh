@@ -73,20 +73,31 @@ __device__ __forceinline__ float2 half2_floats(uint32_t h) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
-// 8 consecutive elements of a row in float32.
+// 8 consecutive elements of a row as they are stored, and in float32.
 template <int DT>
-__device__ __forceinline__ void load8(const void* base, long i, float (&f)[8]) {
-  if (DT == kF32) {
-    const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + i);
-    const float4 a = __ldg(p), b = __ldg(p + 1);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  } else {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(base) + i));
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+struct Raw8 {
+  uint4 v[DT == kF32 ? 2 : 1];
+};
+
+template <int DT>
+__device__ __forceinline__ Raw8<DT> load_raw8(const void* base, long i) {
+  Raw8<DT> r;
+  const char* p = reinterpret_cast<const char*>(base) + i * (DT == kF32 ? 4 : 2);
+  r.v[0] = dev::ld_nc_v4(p);
+  if (DT == kF32) r.v[DT == kF32 ? 1 : 0] = dev::ld_nc_v4(p + 16);
+  return r;
+}
+
+template <int DT>
+__device__ __forceinline__ void floats8(const Raw8<DT>& r, float (&f)[8]) {
+#pragma unroll
+  for (int k = 0; k < (DT == kF32 ? 2 : 1); ++k) {
+    const uint32_t w[4] = {r.v[k].x, r.v[k].y, r.v[k].z, r.v[k].w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (DT == kBF16) {
+      if (DT == kF32) {
+        f[(4 * k + j) % 8] = __uint_as_float(w[j]);
+      } else if (DT == kBF16) {
         f[2 * j] = dev::bf16_lo(w[j]);
         f[2 * j + 1] = dev::bf16_hi(w[j]);
       } else {
@@ -96,6 +107,11 @@ __device__ __forceinline__ void load8(const void* base, long i, float (&f)[8]) {
       }
     }
   }
+}
+
+template <int DT>
+__device__ __forceinline__ void load8(const void* base, long i, float (&f)[8]) {
+  floats8<DT>(load_raw8<DT>(base, i), f);
 }
 
 __device__ __forceinline__ uint32_t pack16(int dtype, float a, float b) {

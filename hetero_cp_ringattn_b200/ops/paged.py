@@ -99,7 +99,7 @@ def rope_append_kv8(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos
     if not qkv.is_cuda:
         return pref.rope_append_kv8(qkv, cos, sin, pos, unit, block_table, k, v, k_scale, v_scale, heads, q_out)
     q = native().rope_append_kv8(qkv, cos, sin, pos, unit, block_table, k, v, k_scale, v_scale, heads, q_out, status)
-    launches.count()
+    launches.count(2 if qkv.shape[0] >= 4 * unit.shape[0] > 0 else 1)   # prompts: k and v, then q
     return q
 
 

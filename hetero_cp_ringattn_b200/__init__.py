@@ -8,10 +8,11 @@ and the tcgen05 attention kernel reads them from local memory. Decode attention 
 partial (O, LSE) over the local shard and combines them across ranks with peer stores.
 
 Sub-packages:
-  models/    Llama/Qwen2 engine (LlamaCPEngine), HF safetensors weights, sampling, fp32 oracle
+  models/    Llama/Qwen2 engine (LlamaCPEngine), single-rank decoder over the 8-bit KV cache
+             (PagedDecoder), HF safetensors weights, sampling, fp32 oracle
   ops/       Python front-ends of the sm_100a kernels (+ fp32/fp64 reference oracles)
   parallel/  capacity chunking, ring layouts, KV-growth schedule (bindings of the host library)
-  kv/        paged, position-tagged KV arena bookkeeping
+  kv/        paged, position-tagged KV arena bookkeeping; the paged 8-bit KV cache
   serve/     control protocol, coordinator, scheduler, worker loop, HTTP API
   utils/     perf JSONL, CUDA-event timing, clock sampling
 Native code: `_C` (sm_100a kernels + the domain runtime), `_host` (C++ host runtime library).
@@ -25,6 +26,8 @@ __version__ = "0.1.0"
 
 _EXPORTS = {
     "LlamaCPEngine": ("models.llama", "LlamaCPEngine"),
+    "PagedDecoder": ("models.paged", "PagedDecoder"),
+    "Kv8Cache": ("kv.quant", "Kv8Cache"),
     "ModelWeights": ("models.weights", "ModelWeights"),
     "PreparedWeights": ("models.weights", "PreparedWeights"),
     "ModelConfig": ("config", "ModelConfig"),

@@ -4,7 +4,8 @@ Parity: the reference's single binary with modes (rust/src/cli.rs:14-165, lib.rs
   * `correctness` - the ring-vs-dense oracle suite with tolerance tiers and a JSON report
     (`--report-path`, `--tolerance-tier`, `--stress-test`; lib.rs:107-199);
   * `infer` - single-node inference with `--export-logits` in the reference's binary layout
-    ([vocab u64 LE][steps u64 LE] then f32 rows; rust/src/infer.rs:74-79);
+    ([vocab u64 LE][steps u64 LE] then f32 rows; rust/src/infer.rs:74-79); `--kv-cache e4m3|int8` runs
+    it on the paged 8-bit KV cache with top-k / top-p / min-p sampling on the device;
   * `serve` - coordinator + workers: one torchrun job, rank 0 coordinates and serves the HTTP API
     (`/v1/completions`, `/health`, `/metrics`), every rank runs the worker command loop
     (coordinator.rs:76-273 and worker.rs:77-143 flags that still apply on one NVSwitch box:
@@ -134,6 +135,8 @@ def cmd_infer(args) -> int:
         tok0 = load_tokenizer(args.model_dir, cfg0.vocab_size)
         text = open(args.prompt_file).read() if args.prompt_file else (args.prompt or "hello")
         return _debug_exports(args, dev, torch.tensor(tok0.encode(text), dtype=torch.int64))
+    if args.kv_cache != "bf16":
+        return _infer_paged(args, dev)
     import torch.distributed as dist
     from .models.sampling import sample_token
     from .parallel.capacity import chunk_sizes
@@ -185,6 +188,29 @@ def cmd_infer(args) -> int:
         eng.close()
         if world > 1:
             dist.destroy_process_group()
+    return 0
+
+
+def _infer_paged(args, dev) -> int:
+    """infer --kv-cache e4m3|int8: one rank, the paged 8-bit KV cache, sampling on the device."""
+    from .models.paged import PagedDecoder
+    from .serve.tokenizer import load_tokenizer
+    if int(os.environ.get("WORLD_SIZE", "1")) != 1:
+        raise SystemExit("--kv-cache e4m3|int8 runs on one rank")
+    if args.export_logits:
+        raise SystemExit("--export-logits needs --kv-cache bf16")
+    cfg, w = _load_model(args, dev)
+    tok = load_tokenizer(args.model_dir, cfg.vocab_size)
+    text = open(args.prompt_file).read() if args.prompt_file else (args.prompt or "hello")
+    ids = torch.tensor(tok.encode(text), dtype=torch.int64)
+    dec = PagedDecoder(cfg, w, rows=1, max_context=max(args.max_context, ids.numel() + args.max_tokens),
+                       kv_cache=args.kv_cache, page=args.kv_page, pages=-(-(ids.numel() + args.max_tokens) // args.kv_page),
+                       device=dev)
+    out = dec.generate([ids], max(1, args.max_tokens), temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
+                       min_p=args.min_p, seed=args.seed)[0].tolist()
+    dec.check_device()
+    print(json.dumps({"prompt_tokens": ids.numel(), "tokens": out, "text": tok.decode(out), "kv_cache": args.kv_cache,
+                      "kv_bytes": dec.cache.bytes}))
     return 0
 
 
@@ -457,6 +483,13 @@ def build_parser() -> argparse.ArgumentParser:
     i.add_argument("--export-logits", default=None)
     i.add_argument("--temperature", type=float, default=0.0)
     i.add_argument("--top-p", type=float, default=1.0)
+    i.add_argument("--kv-cache", default="bf16", choices=["bf16", "e4m3", "int8"],
+                   help="KV cache type; the 8-bit ones run on one rank")
+    i.add_argument("--kv-page", type=int, default=64, choices=[16, 32, 64, 128],
+                   help="tokens per page and scale of an 8-bit KV cache")
+    i.add_argument("--top-k", type=int, default=0, help="keep the k most likely tokens (8-bit KV cache; 0: all)")
+    i.add_argument("--min-p", type=float, default=0.0,
+                   help="keep tokens of at least this share of the most likely one's probability (8-bit KV cache)")
     i.add_argument("--num-domains", type=int, default=None,
                    help="expected number of ranks (checked against WORLD_SIZE)")
     i.add_argument("--chunk-sizes", default=None)

@@ -18,7 +18,8 @@ cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 void check_array(const Tensor& t, const char* name, torch::ScalarType type, int64_t dim, const torch::Device& dev) {
   TORCH_CHECK(t.device() == dev, name, " must be on ", dev);
   TORCH_CHECK(t.scalar_type() == type, name, " must be ", type);
-  TORCH_CHECK(t.dim() == dim && t.is_contiguous(), name, " must be a contiguous ", dim, "-d tensor");
+  // (numbers in messages as text: streaming them into the check's message crashed with this torch build)
+  TORCH_CHECK(t.dim() == dim && t.is_contiguous(), name, " must be a contiguous ", std::to_string(dim), "-d tensor");
 }
 
 int dtype_of(const Tensor& t, const char* name, bool f32) {
@@ -92,7 +93,7 @@ void plan_step(const Tensor& add, const Tensor& kv_len, const Tensor& table, con
   TORCH_CHECK(counters.size(0) == 2 && counters_out.size(0) == 2 && info.size(0) == 4, "counters must have 2 entries, info 4");
   TORCH_CHECK(page >= 1 && page <= (1 << 20), "page must be 1 to 2^20 tokens");
   TORCH_CHECK(R <= hcp::kv8::kPlanMaxRows && T < (1ll << 31) && table.size(1) < (1ll << 31) && ring.size(0) < (1ll << 31),
-              "plan_step: at most ", hcp::kv8::kPlanMaxRows, " rows, and every size below 2^31");
+              "plan_step: at most ", std::to_string(hcp::kv8::kPlanMaxRows), " rows, and every size below 2^31");
   TORCH_CHECK(unit.size(0) >= std::min(T, T / page + 2 * R), "unit must have min(tokens, tokens / page + 2 rows) entries");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(row.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(pos.data_ptr()) % 16 == 0 &&
                   reinterpret_cast<uintptr_t>(slot.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(unit.data_ptr()) % 16 == 0,

@@ -628,8 +628,9 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
       }
       if (kShared) team_sync<kTeam>(stream);
       // ---- O^T += V^T P^T. In a step that ends inside the rows some query token sees, every query
-      // token gets a pass of its own with the codes it must not see taken as 0: whatever a masked
-      // place holds (stale bytes behind the end, NaN in a later draft's row), p = 0 cannot cancel it.
+      // token gets a pass of its own with the codes it must not see taken as 0, and only its own
+      // columns take the result: whatever a masked place holds (stale bytes behind the end, NaN in a
+      // later draft's row), p = 0 cannot cancel it.
       auto values = [&](int q, int seen, bool all) {
         const uint32_t vbase = ring_at + stage_at(q) * kBytes + kTile * D;
 #pragma unroll
@@ -644,9 +645,12 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
               b0[t] = pf[mt][t][0];
               b1[t] = pf[mt][t][1];
             }
-            // column j of the operand is query row t * 8 + j: only this pass's rows
-            if (!all && (n - qn + (r0 + t * 8 + j) / G + 1) != seen) b0[t] = b1[t] = 0u;
           }
+          bool mine[NT][2];   // the lane's accumulator columns that take part in this pass
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) mine[t][i] = all || n - qn + (r0 + t * 8 + 2 * c + i) / G + 1 == seen;
           const int tok = base + q * kTile + mt * 16 + 2 * c;
 #pragma unroll
           for (int k = 0; k < kOut; k += 2) {
@@ -666,7 +670,18 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
               decode4<INT8>(__byte_perm(r[2 * h], 0, 0x3120), af[0], af[1]);
               decode4<INT8>(__byte_perm(r[2 * h + 1], 0, 0x3120), af[2], af[3]);
 #pragma unroll
-              for (int t = 0; t < NT; ++t) mma_f16(acc[k + h][t], af, b0[t], b1[t]);
+              for (int t = 0; t < NT; ++t) {
+                if (all) {
+                  mma_f16(acc[k + h][t], af, b0[t], b1[t]);
+                } else {
+                  float v[4];
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) v[i] = acc[k + h][t][i];
+                  mma_f16(v, af, b0[t], b1[t]);
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) acc[k + h][t][i] = mine[t][i & 1] ? v[i] : acc[k + h][t][i];
+                }
+              }
             }
           }
         }

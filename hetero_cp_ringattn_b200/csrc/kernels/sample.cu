@@ -50,16 +50,37 @@ constexpr int kMaxSlice = 45056;    // floats of a row in one CTA's shared memor
 constexpr int kPairSlice = 20480;   // and where two CTAs share an SM
 constexpr u64 kAll = ~0ull;
 
-// The fixed operations of the weight: no contraction, no flush of subnormals, whatever the flags.
-__device__ __forceinline__ float add_rn(float a, float b) {
+// Operations on logits and distances: no contraction, no flush of subnormals, whatever the flags.
+__device__ __forceinline__ float sub_rn(float a, float b) {
   float r;
-  asm("add.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("sub.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 __device__ __forceinline__ float div_rn(float a, float b) {
   float r;
   asm("div.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
+}
+
+__device__ __forceinline__ float max_rn(float a, float b) {   // (a NaN operand: the other one)
+  float r;
+  asm("max.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float min_rn(float a, float b) {
+  float r;
+  asm("min.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ bool equal(float a, float b) {
+  uint32_t r;
+  asm("{\n\t.reg .pred p;\n\tsetp.eq.f32 p, %1, %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r) : "f"(a), "f"(b));
+  return r != 0;
+}
+__device__ __forceinline__ float warp_max_rn(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = max_rn(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
 }
 
 // floor(2^31 exp(-d)) for 0 <= d <= 64: y = d log2(e), n = round(y), 2^(n - y) on [-1/2, 1/2] by the
@@ -190,18 +211,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
         const float4 q = make_float4(bf16_lo(v.z), bf16_hi(v.z), bf16_lo(v.w), bf16_hi(v.w));
         x4[2 * i] = p;
         x4[2 * i + 1] = q;
-        top = fmaxf(top, fmaxf(fmaxf(fmaxf(p.x, p.y), fmaxf(p.z, p.w)), fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w))));
+        top = max_rn(top, max_rn(max_rn(max_rn(p.x, p.y), max_rn(p.z, p.w)), max_rn(max_rn(q.x, q.y), max_rn(q.z, q.w))));
       } else {
         const float4 p = make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
         x4[i] = p;
-        top = fmaxf(top, fmaxf(fmaxf(p.x, p.y), fmaxf(p.z, p.w)));
+        top = max_rn(top, max_rn(max_rn(p.x, p.y), max_rn(p.z, p.w)));
       }
     }
     for (int i = nv * vec + tid; i < n; i += kThreads) {
       const float f = BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(src)[i])
                            : reinterpret_cast<const float*>(src)[i];
       x[i] = f;
-      top = fmaxf(top, f);
+      top = max_rn(top, f);
     }
   }
   const float temp = a.temperature.ptr ? a.temperature.ptr[b] : a.temperature.value;
@@ -216,16 +237,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
   };
   if (use_k || use_p) clear();
   if (tid == 0) S.list_n = 0;
-  top = warp_max(top);
+  top = warp_max_rn(top);
   float* wf = reinterpret_cast<float*>(S.warp_a);
   if (lane == 0) wf[warp] = top;
   cluster.barrier_wait();
   __syncthreads();
-  top = warp_max(wf[lane % kWarps]);
+  top = warp_max_rn(wf[lane % kWarps]);
   if (tid < C) *cluster.map_shared_rank(&S.fslot[rank], tid) = top;
   cluster.sync();
   top = S.fslot[0];
-  for (int i = 1; i < C; ++i) top = fmaxf(top, S.fslot[i]);
+  for (int i = 1; i < C; ++i) top = max_rn(top, S.fslot[i]);
 
   if (top == ninf) {   // nothing to draw (the whole cluster agrees)
     if (rank == 0 && tid == 0) a.token[b] = -1;
@@ -234,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
   if (greedy) {
     uint32_t best = 0xffffffffu;
     for (int i = s0 + lane; i < s1; i += 32)
-      if (x[i] == top) best = min(best, uint32_t(lo + i));
+      if (equal(x[i], top)) best = min(best, uint32_t(lo + i));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) best = min(best, __shfl_xor_sync(0xffffffffu, best, o));
     if (lane == 0) S.warp_b[warp] = best;
@@ -267,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
   // (top - l) / T, correctly rounded: by the reciprocal and one correction of the quotient (Markstein
   // 1990: with r = RN(1 / T), q = RN(x r) and e = x - q T exact in a fused multiply-add, RN(q + e r)
   // is RN(x / T)) where no step can leave the normal range (a finite top of at least 2^-30 keeps every
-  // nonzero difference above 2^-60); else by division. fminf(NaN, 64) = 64: NaN logits and
+  // nonzero difference above 2^-60); else by division. min(NaN, 64) = 64: NaN logits and
   // infinite distances end beyond every weight.
   const float inv_t = div_rn(1.f, temp);
   const bool by_inverse = temp >= 0x1p-60f && temp <= 0x1p60f && fabsf(top) >= 0x1p-30f && fabsf(top) < 3.4e38f;
@@ -277,9 +298,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
       const float2 r = make_float2(inv_t, inv_t), q = __fmul2_rn(v, r);
       const float2 e = __ffma2_rn(make_float2(-q.x, -q.y), make_float2(temp, temp), v);
       const float2 d = __ffma2_rn(e, r, q);
-      return make_float2(fminf(d.x, 64.f), fminf(d.y, 64.f));
+      return make_float2(min_rn(d.x, 64.f), min_rn(d.y, 64.f));
     }
-    auto one = [&](float v) { return v == top ? 0.f : fminf(div_rn(add_rn(top, -v), temp), 64.f); };
+    auto one = [&](float v) { return equal(v, top) ? 0.f : min_rn(div_rn(sub_rn(top, v), temp), 64.f); };
     return make_float2(one(l.x), one(l.y));
   };
   u64 sum = 0;                // without a filter: of the kept weights

@@ -331,38 +331,37 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
     }
     z.pp = pp;
   };
-  auto copy = [&](int put_stage, int put_tile, int tiles) {
-    if (lane >= kStep * halves) return;
-    const int my_tile = lane / halves, my_half = lane % halves;
-    const int ahead = my_tile >= put_tile ? my_tile - put_tile : my_tile - put_tile + kStep;
-    if (ahead >= tiles) return;
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    CopyLane& z = s_copy[stream][lane];
-    if (!z.tile) return;
-    const int st = put_stage + ahead >= kStages ? put_stage + ahead - kStages : put_stage + ahead;
+  // K, V and the scales of one page of a tile into a stage; without a page only the arrival
+  auto issue = [&](int st, int half, bool valid, int page, int row, int h) {
     uint64_t* bar = &bars[stream][st];
-    const bool valid = z.valid != 0;
-    const int page = z.page;
-    // bytes of the lane's own page: the barrier counts the lanes
     const int box = min(P, kTile);
-    float* sc = meta[stream][st][my_half];
+    float* sc = meta[stream][st][half];
     if (valid) {
       mbar_expect_tx(bar, 2u * uint32_t(box) * D);
-      unsigned char* dst = ring + st * kBytes + my_half * 16 * D;
+      unsigned char* dst = ring + st * kBytes + half * 16 * D;
       // a page id outside the pool reads as zeros (the tensor map's bounds)
-      tma_load_4d(dst, &kmap, bar, z.row, z.h, page);
-      tma_load_4d(dst + kTile * D, &vmap, bar, z.row, z.h, page);
+      tma_load_4d(dst, &kmap, bar, row, h, page);
+      tma_load_4d(dst + kTile * D, &vmap, bar, row, h, page);
     }
     if (valid && page >= 0 && page < a.c.pages) {
-      const long at = (long)page * a.c.scale_page_stride + (long)z.h * a.c.scale_head_stride;
+      const long at = (long)page * a.c.scale_page_stride + (long)h * a.c.scale_head_stride;
       asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(sc)), "l"(a.c.k_scale + at) : "memory");
       asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(sc + 1)), "l"(a.c.v_scale + at) : "memory");
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
     } else {
-      if (valid) report_error(a.status, int(StatusCode::kOutOfBounds), 411, page, z.h);
+      if (valid) report_error(a.status, int(StatusCode::kOutOfBounds), 411, page, h);
       sc[0] = sc[1] = 1.f;
       mbar_arrive(bar);
     }
+  };
+  auto copy = [&](int put_stage, int put_tile, int tiles) {
+    if (lane >= kStep * halves) return;
+    const int my_tile = lane / halves, my_half = lane % halves;
+    const int ahead = my_tile >= put_tile ? my_tile - put_tile : my_tile - put_tile + kStep;
+    CopyLane& z = s_copy[stream][lane];
+    if (ahead >= tiles || !z.tile) return;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    issue(put_stage + ahead >= kStages ? put_stage + ahead - kStages : put_stage + ahead, my_half, z.valid != 0, z.page, z.row, z.h);
     const long long px = z.px + kStep;
     Place pp = z.pp;
     pp.tile += kStep;
@@ -370,12 +369,22 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
     look_up(z, px, pp, my_half);
   };
   if (copies && x0 < x1) {
+    // the first tiles, every page by a lane of its own, so that their look-ups are one latency
+    for (int e = lane; e < kStages * halves; e += 32) {
+      const int half = e % halves, st = e / halves;
+      if (x0 + st < x1) {
+        const Place p = place_of(x0 + st);
+        const int block = p.tile * kTile / P + half;
+        const bool valid = block * P < p.n;
+        issue(st, half, valid, valid ? a.table[(long)p.b * a.width + block] : 0, p.tile * kTile % P, p.h);
+      }
+    }
     if (lane < kStep * halves) {
-      const long long px = x0 + lane / halves;
+      // the lane's first tile of those that follow, in its own place modulo kStep
+      const int my_tile = lane / halves;
+      const long long px = x0 + kStages + (my_tile + kStep - kStages % kStep) % kStep;
       look_up(s_copy[stream][lane], px, px < x1 ? place_of(px) : Place{}, lane % halves);
     }
-#pragma unroll 1
-    for (int i = 0; i < kStages; i += kStep) copy(i, 0, min(kStep, kStages - i));
   }
   __syncwarp();
 
@@ -794,60 +803,63 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
   __syncthreads();
 
   // ---------------------------------------------------------------- the CTA's pieces, item by item
-  // bit 2 i + k of a mask: piece k of stream i. Every warp finds the items by itself.
+  // bit 2 i + k of a mask: piece k of stream i. Every warp finds the items by itself; the threads share
+  // (item, row, four dims) so that all pieces of all items are read at once.
   const long long my_start = lane < 2 * kStreams ? s_start[lane >> 1][lane & 1] : -1;
   const uint32_t same = __match_any_sync(0xffffffffu, my_start);
-  uint32_t leaders = __ballot_sync(0xffffffffu, my_start >= 0 && __ffs(same) - 1 == lane);
-  bool open = false;
-  while (leaders) {
-    const int lead = __ffs(leaders) - 1;
-    leaders &= leaders - 1;
+  const uint32_t leaders = __ballot_sync(0xffffffffu, my_start >= 0 && __ffs(same) - 1 == lane);
+  const int items = __popc(leaders);
+  constexpr int kElems = kRows * (D / 4);     // of an item (a multiple of a warp: a warp's lanes share an item)
+  for (int at = tid; at < items * kElems; at += kWarps * 32) {
+    const int lead = __fns(leaders, 0, at / kElems + 1);
     const uint32_t mask = __shfl_sync(0xffffffffu, same, lead);
     const long long start = __shfl_sync(0xffffffffu, my_start, lead);
     const Place& p = s_place[lead >> 1][lead & 1];
-    const int tiles = p.tiles, h = p.h, first = p.first;
+    const int r = at % kElems / (D / 4), d = at % (D / 4);
     const int r0 = p.rt * kRows, rows = min(p.qn * G - r0, kRows);
-    const bool inside = start >= c0 && start + tiles <= c1;
-    const int piece_at = start < c0 ? 0 : 1;
-    if (!inside && piece_at == 1) {
-      open = true;
-      if (tid == 0) ws.straddle[blockIdx.x] = Straddle{ctas.part_of(start + tiles - 1), r0, rows, first, h * G, {0, 0, 0}};
-    }
-    for (int at = tid; at < rows * (D / 4); at += kWarps * 32) {
-      const int r = at / (D / 4), d = at % (D / 4);
-      float top = kNone;
+    if (r >= rows) continue;
+    float top = kNone;
 #pragma unroll
-      for (int k = 0; k < 2 * kStreams; ++k)
-        if (mask >> k & 1) top = fmaxf(top, s_ml[k >> 1][k & 1][r][0]);
-      float l = 0.f;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      auto add = [&](int k, const float4 o) {
-        const float w = fast_exp2(s_ml[k >> 1][k & 1][r][0] - top);
-        l = fmaf(w, s_ml[k >> 1][k & 1][r][1], l);
-        v.x = fmaf(w, o.x, v.x);
-        v.y = fmaf(w, o.y, v.y);
-        v.z = fmaf(w, o.z, v.z);
-        v.w = fmaf(w, o.w, v.w);
-      };
+    for (int k = 0; k < 2 * kStreams; ++k)
+      if (mask >> k & 1) top = fmaxf(top, s_ml[k >> 1][k & 1][r][0]);
+    float l = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](int k, const float4 o) {
+      const float w = fast_exp2(s_ml[k >> 1][k & 1][r][0] - top);
+      l = fmaf(w, s_ml[k >> 1][k & 1][r][1], l);
+      v.x = fmaf(w, o.x, v.x);
+      v.y = fmaf(w, o.y, v.y);
+      v.z = fmaf(w, o.z, v.z);
+      v.w = fmaf(w, o.w, v.w);
+    };
 #pragma unroll
-      for (int k = 0; k < 2 * kStreams; ++k)
-        if (mask >> k & 1)
-          add(k, (k & 1) ? *reinterpret_cast<const float4*>(ring_base + (k >> 1) * S::kRing + ((size_t)r * D + 4 * d) * 4)
-                         : *reinterpret_cast<const float4*>(ws.head + (((size_t)blockIdx.x * kStreams + (k >> 1)) * kRows + r) * D + 4 * d));
-      if (inside) {
-        const int qi = (r0 + r) / G, head = h * G + (r0 + r) % G;
-        const float inv = row_inv(l);
-        reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.o) + ((long)(first + qi) * a.H + head) * D)[d] =
-            make_uint2(pack16(a.q_dtype, v.x * inv, v.y * inv), pack16(a.q_dtype, v.z * inv, v.w * inv));
-        if (d == 0 && a.lse != nullptr) a.lse[(long)head * a.T + first + qi] = row_lse(top, l);
-      } else {
-        const size_t row = ((size_t)blockIdx.x * 2 + piece_at) * kRows + r;
-        reinterpret_cast<float4*>(ws.o + row * D)[d] = v;
-        if (d == 0) *reinterpret_cast<float2*>(ws.ml + row * 2) = make_float2(top, l);
-      }
+    for (int k = 0; k < 2 * kStreams; ++k)
+      if (mask >> k & 1)
+        add(k, (k & 1) ? *reinterpret_cast<const float4*>(ring_base + (k >> 1) * S::kRing + ((size_t)r * D + 4 * d) * 4)
+                       : *reinterpret_cast<const float4*>(ws.head + (((size_t)blockIdx.x * kStreams + (k >> 1)) * kRows + r) * D + 4 * d));
+    if (start >= c0 && start + p.tiles <= c1) {
+      const int qi = (r0 + r) / G, head = p.h * G + (r0 + r) % G;
+      const float inv = row_inv(l);
+      reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.o) + ((long)(p.first + qi) * a.H + head) * D)[d] =
+          make_uint2(pack16(a.q_dtype, v.x * inv, v.y * inv), pack16(a.q_dtype, v.z * inv, v.w * inv));
+      if (d == 0 && a.lse != nullptr) a.lse[(long)head * a.T + p.first + qi] = row_lse(top, l);
+    } else {
+      const size_t row = ((size_t)blockIdx.x * 2 + (start < c0 ? 0 : 1)) * kRows + r;
+      reinterpret_cast<float4*>(ws.o + row * D)[d] = v;
+      if (d == 0) *reinterpret_cast<float2*>(ws.ml + row * 2) = make_float2(top, l);
     }
   }
-  if (!open && tid == 0) ws.straddle[blockIdx.x].last = -1;
+  if (warp == 0) {
+    // the item that starts in this range and goes on past it, if there is one
+    const bool open = (leaders >> lane & 1) && my_start >= c0 && my_start + s_place[lane >> 1][lane & 1].tiles > c1;
+    const uint32_t who = __ballot_sync(0xffffffffu, open);
+    if (open) {
+      const Place& p = s_place[lane >> 1][lane & 1];
+      const int r0 = p.rt * kRows;
+      ws.straddle[blockIdx.x] = Straddle{ctas.part_of(my_start + p.tiles - 1), r0, min(p.qn * G - r0, kRows), p.first, p.h * G, {0, 0, 0}};
+    }
+    if (who == 0 && lane == 0) ws.straddle[blockIdx.x].last = -1;
+  }
 }
 
 // One CTA per (CTA of the attention, query row): where that CTA's last item goes on in the next ones,

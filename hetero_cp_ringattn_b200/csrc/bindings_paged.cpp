@@ -171,13 +171,24 @@ Tensor rope_append_kv8(const Tensor& x, const Tensor& cos_t, const Tensor& sin_t
   return out;
 }
 
-void gather_kv8(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs, const Tensor& table, int64_t n, const Tensor& k_out,
-                const Tensor& v_out) {
+std::tuple<Tensor, Tensor> gather_kv8(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs, const Tensor& table, int64_t n,
+                                      const optional<Tensor>& k_buf, const optional<Tensor>& v_buf) {
   hcp::kv8::GatherArgs a{};
   a.c = cache_of(k, v, ks, vs);
   const auto dev = k.device();
   check_array(table, "block_table row", torch::kInt32, 1, dev);
   TORCH_CHECK(n >= 0 && n < (1ll << 31), "rows to gather out of range");
+  const c10::cuda::CUDAGuard g(dev);
+  TORCH_CHECK(k_buf.has_value() == v_buf.has_value(), "give both output buffers or none");
+  Tensor k_out, v_out;
+  if (k_buf.has_value()) {
+    k_out = *k_buf;
+    v_out = *v_buf;
+  } else {
+    const auto opt = k.options().dtype(torch::kBFloat16);
+    k_out = torch::empty({a.c.Hkv, n, a.c.D}, opt);
+    v_out = torch::empty({a.c.Hkv, n, a.c.D}, opt);
+  }
   for (const Tensor* o : {&k_out, &v_out}) {
     TORCH_CHECK(o->device() == dev && o->scalar_type() == torch::kBFloat16 && o->dim() == 3 && o->size(0) == a.c.Hkv && o->size(1) >= n &&
                     o->size(2) == a.c.D && o->stride(2) == 1 && o->stride(1) == a.c.D && o->stride(0) % 8 == 0 &&
@@ -185,7 +196,6 @@ void gather_kv8(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor
                 "the outputs must be bfloat16 [kv_heads, rows or more, head_dim] with contiguous rows");
   }
   TORCH_CHECK(k_out.strides() == v_out.strides(), "the outputs must have the same strides");
-  const c10::cuda::CUDAGuard g(dev);
   a.table = table.data_ptr<int>();
   a.width = int(table.size(0));
   a.n = int(n);
@@ -193,6 +203,7 @@ void gather_kv8(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor
   a.v_out = v_out.data_ptr();
   a.out_head_stride = k_out.stride(0);
   HCP_CHECK_OK(hcp::kv8::gather(a, cur_stream()));
+  return {k_out, v_out};
 }
 
 std::tuple<Tensor, Tensor> attention_kv8(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs,

@@ -15,7 +15,7 @@
 // are 0; u has 24 bits and cannot reach them.
 //
 // One cluster per row: each CTA holds a contiguous slice of the row in shared memory, so the logits
-// are read from memory once. A histogram over d (bins of 1/64; counts for top-k, counts
+// are read from memory once. A histogram over d (bins of 1/32; counts for top-k, counts
 // and weight sums for top-p) gives the bin where the cut falls; the tokens up to it, usually a few
 // dozen, are sent to one CTA, sorted and finished there. More than 512 of them (a large k, a flat row, ties) take the general way: histograms of the
 // crossing bin until it is small, or the exact tie, then one pass over the kept tokens.
@@ -43,7 +43,8 @@ typedef unsigned long long u64;
 
 constexpr int kThreads = 512;        // two CTAs an SM: one row's barriers hide behind another's work
 constexpr int kWarps = kThreads / 32;
-constexpr int kBins = 2048;
+constexpr int kBins = 1024;
+constexpr float kPerUnit = 32.f;      // bins per unit of d
 constexpr int kList = kThreads;     // tokens that are ordered directly (one a thread)
 constexpr int kMaxCluster = 16;     // 16 is the hardware's limit (above 8: opt-in)
 constexpr int kMaxSlice = 45056;    // floats of a row in one CTA's shared memory
@@ -111,9 +112,9 @@ __device__ __forceinline__ uint2 weight2(float d0, float d1) {
 }
 __device__ __forceinline__ uint32_t weight(float d) { return weight2(d, d).x; }
 
-// floor(64 d), at most kBins - 1 (d <= 64: adding 2^23 towards zero leaves the floor in the low bits).
+// floor(32 d), at most kBins - 1 (d <= 64: adding 2^23 towards zero leaves the floor in the low bits).
 __device__ __forceinline__ int bin_of(float d) {
-  return min(int(__float_as_uint(__fadd_rz(d * 64.f, 8388608.f)) & 0x7fffff), kBins - 1);
+  return min(int(__float_as_uint(__fadd_rz(d * kPerUnit, 8388608.f)) & 0x7fffff), kBins - 1);
 }
 
 // floor(total * x) for x in [0, 1], x held in 24 bits (total < 2^54).
@@ -381,24 +382,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
   // ---------------------------------------------------------------- the bin of the cut
   // The bin where the cluster's count (or weight) reaches `target` (or top_p of the weight in all the
   // bins, for target 0, which it returns). Every CTA sums
-  // one segment of the bins over the cluster (reading all of every histogram in every CTA would take
+  // one segment of the bins (weights only with `sums`) over the cluster (reading all of every histogram in every CTA would take
   // C times the distributed-memory traffic, which is what this costs), the segments' totals say whose
   // segment the crossing is in, and that CTA tells the others.
-  auto find_bin = [&](bool by_weight, u64 target, u64 base_cnt, u64 base_w) {
+  auto find_bin = [&](bool by_weight, u64 target, u64 base_cnt, u64 base_w, bool sums = true) {
     const int per = kBins / C;                 // C is a power of two of at most 16
     const int from = tid % C;
 #pragma unroll
     for (int p = tid; p < kBins; p += kThreads) {
       const int i = p / C;
       const uint2 h = *cluster.map_shared_rank(&S.hist[rank * per + i], from);
-      u64 c = h.x & 0xffffu, w = (u64(h.x >> 16) << 32) + h.y;
-      for (int o = C >> 1; o > 0; o >>= 1) {
-        c += __shfl_xor_sync(0xffffffffu, c, o);
-        w += __shfl_xor_sync(0xffffffffu, w, o);
-      }
-      if (from == 0) {
-        seg_c[i] = uint32_t(c);
-        seg_w[i] = w;
+      uint32_t c = h.x & 0xffffu;
+      for (int o = C >> 1; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+      if (from == 0) seg_c[i] = c;
+      if (sums) {
+        u64 w = (u64(h.x >> 16) << 32) + h.y;
+        for (int o = C >> 1; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+        if (from == 0) seg_w[i] = w;
       }
     }
     __syncthreads();
@@ -408,10 +408,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
       const int i = tid * mine_n + j;
       if (i < per) {
         tc += seg_c[i];
-        tw += seg_w[i];
+        if (sums) tw += seg_w[i];
       }
     }
-    const u64 ic = warp_scan64(tc, lane), iw = warp_scan64(tw, lane);
+    const u64 ic = warp_scan64(tc, lane), iw = sums ? warp_scan64(tw, lane) : 0;
     if (lane == 31) {
       S.warp_a[warp] = ic;
       S.warp_b[warp] = iw;
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     __syncthreads();
     const u64 oc = lane < kWarps ? S.warp_a[lane] : 0, ow = lane < kWarps ? S.warp_b[lane] : 0;
     if (warp == 0) {
-      const u64 t0 = warp_sum64(oc), t1 = warp_sum64(ow);
+      const u64 t0 = warp_sum64(oc), t1 = sums ? warp_sum64(ow) : 0;
       if (lane < C) {
         *cluster.map_shared_rank(&S.slot_c[rank], lane) = t0;
         *cluster.map_shared_rank(&S.slot_w[rank], lane) = t1;
@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     }
     publish();
     u64 ec = base_cnt + ic - tc + warp_sum64(lane < warp ? oc : 0);
-    u64 ew = base_w + iw - tw + warp_sum64(lane < warp ? ow : 0);
+    u64 ew = base_w + (sums ? iw - tw + warp_sum64(lane < warp ? ow : 0) : 0);
     u64 all_w = 0;
     for (int r = 0; r < C; ++r) {
       if (r < rank) {
@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     for (int j = 0; j < mine_n; ++j) {
       const int i = tid * mine_n + j;
       if (i >= per) break;
-      const u64 c = seg_c[i], w = seg_w[i];
+      const u64 c = seg_c[i], w = sums ? seg_w[i] : 0;
       const u64 before = by_weight ? ew : ec, in = by_weight ? w : c;
       if (before < target && before + in >= target) {
         for (int r = 0; r < C; ++r) {
@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
   };
   bool by_k = use_k;
   publish();                   // the histograms are complete
-  u64 limit = find_bin(!by_k, by_k ? u64(top_k) : 0, 0, 0);
+  u64 limit = find_bin(!by_k, by_k ? u64(top_k) : 0, 0, 0, !by_k);
   if (by_k && (S.found_bin < 0 || S.found_bin == kBins - 1)) {
     // the last bin holds only weights of 0: a top-k cut inside it leaves the draw as it is
     by_k = false;
@@ -479,12 +479,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
   const bool cut_somewhere = by_k || use_p;
   int bin = S.found_bin;
   u64 bin_cnt = S.found_cnt, bin_w = S.found_w, bin_in = S.found_in_cnt;
-  // the first level's bin b holds the keys of d in [b / 64, (b + 1) / 64)
-  auto first_lo = [](int i) { return __float_as_uint(float(i) * (1.f / 64.f)); };
+  // the first level's bin b holds the keys of d in [b / 32, (b + 1) / 32)
+  auto first_lo = [](int i) { return __float_as_uint(float(i) * (1.f / kPerUnit)); };
 
   // ---------------------------------------------------------------- few tokens up to it: one CTA's work
   if (cut_somewhere && bin >= 0 && bin_cnt + bin_in <= kList) {
-    const float end = float(bin + 1) * (1.f / 64.f);
+    const float end = float(bin + 1) * (1.f / kPerUnit);
     Shared* to = cluster.map_shared_rank(&S, 0);
     auto send = [&](float d, int i) {
       if (d < end) to->all[atomicAdd(&to->list_n, 1)] = (u64(__float_as_uint(d)) << 32) | uint32_t(lo + i);

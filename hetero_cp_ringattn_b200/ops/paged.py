@@ -131,12 +131,10 @@ def gather_kv8(k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale:
                out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """The first n cached rows of one request as bf16 K and V [kv_heads, n or more, D] in position order,
     what `kernels.attention` reads. `out`: buffers to write into."""
-    if out is None:
-        shape = (k.shape[1], n, k.shape[3])
-        out = (torch.empty(shape, dtype=torch.bfloat16, device=k.device),
-               torch.empty(shape, dtype=torch.bfloat16, device=k.device))
     if not k.is_cuda:
+        if out is None:
+            out = tuple(torch.empty(k.shape[1], n, k.shape[3], dtype=torch.bfloat16) for _ in "kv")
         return pref.gather_kv8(k, v, k_scale, v_scale, block_table_row, n, out)
-    native().gather_kv8(k, v, k_scale, v_scale, block_table_row, n, out[0], out[1])
+    out = native().gather_kv8(k, v, k_scale, v_scale, block_table_row, n, *(out or (None, None)))
     launches.count()
     return out

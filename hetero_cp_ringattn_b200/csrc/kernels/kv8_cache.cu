@@ -11,7 +11,11 @@
 // gather: the first n cached rows of a request as position-ordered bf16 [Hkv][n][D], the layout
 // the prefill attention reads.
 //
-// Both are bound by memory traffic.
+// Both are bound by memory traffic, the append of a few tokens by latency. Measured on B200 with 32
+// query heads, 8 KV heads, 128 dims, pages of 64: append of 16381 tokens 80 us (369 MB, 4.6 TB/s: q's
+// half 47 us at 5.7 TB/s, k and v 33 us, their chain of loads, block maximum and codes), of one token
+// to each of 64 rows 8 us; gather of 131072 rows 133 us (805 MB, 6.0 TB/s, 92% of a plain copy's rate),
+// of 2041 rows with 2 KV heads 6 us.
 #include "kv8_common.cuh"
 #include "launch.h"
 
@@ -286,7 +290,8 @@ __global__ void __launch_bounds__(kThreads, 4) append_short_kernel(AppendArgs a,
 }
 
 // Prompts: two launches, since the two want different shapes: k and v 128 registers a thread for what
-// they hold and prefetch, q as many threads as there are.
+// they hold and prefetch, q as many threads as there are. (16381 tokens: 80 us; one launch of both 88;
+// k and v with 16 values a thread, twice the threads and 64 registers, 91.)
 template <int DT, int D, bool INT8>
 __global__ void __launch_bounds__(512, 1) append_block_kernel(AppendArgs a, int heads) {
   pdl_trigger();

@@ -11,7 +11,9 @@
 // write. New pages are looked up by their place in the ring rather than through the table, so no CTA
 // depends on an entry that another one writes. Where the new lengths or counters overwrite the old
 // ones, the CTAs form one cluster (of at most 8) whose barrier separates the reads of the state from
-// its update; otherwise there are as many CTAs as the writes are worth.
+// its update; otherwise there are as many CTAs as the writes are worth. Measured on B200, caches cold:
+// 64 rows growing by a token 10 us with 1 to 64 CTAs; 509 rows with 131072 new tokens (2 MB written)
+// 135 us with one CTA, 25 with 8, 14 with 32 or more.
 #include <cooperative_groups.h>
 
 #include "common.cuh"

@@ -15,12 +15,17 @@
 // are 0; u has 24 bits and cannot reach them.
 //
 // One cluster per row: each CTA holds a contiguous slice of the row in shared memory, so the logits
-// are read from memory once. A histogram over d (bins of 1/32; counts for top-k, counts
-// and weight sums for top-p) gives the bin where the cut falls; the tokens up to it, usually a few
-// dozen, are sent to one CTA, sorted and finished there. More than 512 of them (a large k, a flat row, ties) take the general way: histograms of the
-// crossing bin until it is small, or the exact tie, then one pass over the kept tokens.
+// are read from memory once. A histogram over d (bins of 1/32; counts for top-k, counts and weight
+// sums for top-p) gives the bin where the cut falls; the tokens up to it, usually a few dozen, are
+// sent to one CTA, sorted and finished there. More than 512 of them (a large k, a flat row, ties) take
+// the general way: histograms of the crossing bin until it is small, or the exact tie, then one pass
+// over the kept tokens.
+//
 // Bound: instructions per token (distance, weight) for many rows, the chain of cluster barriers for
-// one. The weight's polynomial runs on packed pairs.
+// one. The weight's polynomial runs on packed pairs. Measured on B200, float32 logits: one row of
+// 128256 tokens 20 us; 129 rows of 151936 (78 MB, 12 us of reading) 102 us with mixed settings, greedy
+// alone 32, temperature alone 62, top-k 40 83, top-k 1000 115, top-p 0.9 over random logits (the
+// general way) 179. One CTA a row that reads the row again in every pass instead of holding it: 289.
 #include <cooperative_groups.h>
 
 #include <cuda_bf16.h>

@@ -240,7 +240,7 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
   __shared__ long long s_start[kStreams][2];               // first tile of the piece's item; -1: no piece
   __shared__ Place s_place[kStreams][2];
   __shared__ float s_max[kShared ? kStreams : 1][kTeam][kRows];   // team: the warps' column maxima
-  __shared__ uint32_t s_p[kShared ? kStreams : 1][2 * kStep][kShared ? NT * 2 : 1][32];   // team: P^T of each 16 tokens
+  __shared__ uint2 s_p[kShared ? kStreams : 1][2 * kStep][kShared ? NT : 1][32];   // team: P^T of each 16 tokens
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int stream = warp / kTeam, sub = warp % kTeam;
   const int G = a.H / a.c.Hkv, P = a.c.P, Hkv = a.c.Hkv;
@@ -554,11 +554,15 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
         dead[mt] = vs == 0.f || idle;
         const float lv = dead[mt] ? 0.f : __log2f(vs);
         iv[mt] = dead[mt] ? 1.f : __fdividef(1.f, vs);
-        const float f = factor * ks;
+        const float2 f = make_float2(factor * ks, factor * ks), lv2 = make_float2(lv, lv);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[mt][t][i] = fmaf(s[mt][t][i], f, lv);
+          for (int i = 0; i < 4; i += 2) {
+            const float2 x = __ffma2_rn(make_float2(s[mt][t][i], s[mt][t][i + 1]), f, lv2);
+            s[mt][t][i] = x.x;
+            s[mt][t][i + 1] = x.y;
+          }
       }
       if (edge) {
 #pragma unroll
@@ -580,7 +584,7 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
         for (int i = 0; i < 2; ++i) {
           float v = fmaxf(s[0][t][i], s[0][t][i + 2]);
 #pragma unroll
-          for (int mt = 1; mt < kMt; ++mt) v = fmaxf(v, fmaxf(s[mt][t][i], s[mt][t][i + 2]));
+          for (int mt = 1; mt < kMt; ++mt) v = max3f(v, s[mt][t][i], s[mt][t][i + 2]);
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
           top[t][i] = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
@@ -620,29 +624,41 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
 #pragma unroll
           for (int k = 0; k < kOut; ++k)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[k][t][i] *= up[i & 1];
+            for (int i = 0; i < 4; i += 2) {
+              const float2 x = __fmul2_rn(make_float2(acc[k][t][i], acc[k][t][i + 1]), make_float2(up[0], up[1]));
+              acc[k][t][i] = x.x;
+              acc[k][t][i + 1] = x.y;
+            }
         }
       }
       // ---- p, its sum, and P^T as the B operand of a 16-token step
       uint32_t pf[kMt][NT][2];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const float mu[2] = {m[t][0] - kShift, m[t][1] - kShift};
+        const float2 up = make_float2(kShift - m[t][0], kShift - m[t][1]);
+        float2 sum = make_float2(l[t][0], l[t][1]);
 #pragma unroll
         for (int mt = 0; mt < kMt; ++mt) {
-          float e[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            e[i] = fast_exp2(s[mt][t][i] - mu[i & 1]);
-            l[t][i & 1] = fmaf(e[i], iv[mt], l[t][i & 1]);
+          for (int i = 0; i < 2; ++i) {
+            const float2 x = __fadd2_rn(make_float2(s[mt][t][2 * i], s[mt][t][2 * i + 1]), up);
+            const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+            sum = __ffma2_rn(e, make_float2(iv[mt], iv[mt]), sum);
+            pf[mt][t][i] = transpose8x8(pack_half(e.x, e.y));
           }
-          const uint32_t lo = pack_half(e[0], e[1]), hi = pack_half(e[2], e[3]);
-          pf[mt][t][0] = transpose8x8(dead[mt] ? 0u : lo);
-          pf[mt][t][1] = transpose8x8(dead[mt] ? 0u : hi);
-          if constexpr (kShared) {
-            s_p[stream][g0 + mt][2 * t][lane] = pf[mt][t][0];
-            s_p[stream][g0 + mt][2 * t + 1][lane] = pf[mt][t][1];
-          }
+        }
+        l[t][0] = sum.x;
+        l[t][1] = sum.y;
+      }
+#pragma unroll
+      for (int mt = 0; mt < kMt; ++mt) {
+        if (dead[mt]) {     // (the same for the warp)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) pf[mt][t][0] = pf[mt][t][1] = 0u;
+        }
+        if constexpr (kShared) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t) s_p[stream][g0 + mt][t][lane] = make_uint2(pf[mt][t][0], pf[mt][t][1]);
         }
       }
       if (kShared) team_sync<kTeam>(stream);
@@ -658,8 +674,9 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             if constexpr (kShared) {
-              b0[t] = s_p[stream][q * 2 + mt][2 * t][lane];
-              b1[t] = s_p[stream][q * 2 + mt][2 * t + 1][lane];
+              const uint2 b = s_p[stream][q * 2 + mt][t][lane];
+              b0[t] = b.x;
+              b1[t] = b.y;
             } else {
               b0[t] = pf[mt][t][0];
               b1[t] = pf[mt][t][1];

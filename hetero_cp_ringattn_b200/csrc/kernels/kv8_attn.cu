@@ -26,10 +26,10 @@
 // is left as (m, l, O) partials that a second small launch combines in list order.
 //
 // Measured on B200, caches cold, cache bytes a second (a plain copy: 6.55 TB/s): 64 requests of up to
-// 32768 rows, 8 KV heads of 128 dims, 4 query rows each: 220 us, 5.8 TB/s e4m3, 5.9 int8; 64 dims: 140
+// 32768 rows, 8 KV heads of 128 dims, 4 query rows each: 222 us, 5.8 TB/s e4m3, 6.1 int8; 64 dims: 140
 // us, 4.7. Small work is latency: one request of 4097 rows 15 us, of 131071 rows 32 us, 33 requests of
 // up to 8192 44 to 48 us (some SMs, those of the larger clusters of SMs, end up to 10% later than
-// others). Five tokens of 7 heads (35 rows): 304 us, where 100 are the bytes: bound by the chain from
+// others). Five tokens of 7 heads (35 rows): 299 us, where 100 are the bytes: bound by the chain from
 // scores to weights to the next products with 8 warps an SM, the tensor cores 38% busy.
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -56,8 +56,9 @@ constexpr float kLn2 = 0.6931471805599453f;
 // accumulates kOut 16-dim pieces of O over all tokens of the step. So up to 40 query rows take one pass
 // over the cache with their accumulators in registers, no code is converted twice, and registers
 // allow the warps that hide each other's latencies (a warp alone issues about every fifth cycle).
-// 12 warps where registers allow it. 35 rows of 128 dims: 304 us; in single warps of 16 rows, three
+// 12 warps where registers allow it. 35 rows of 128 dims: 299 us; in single warps of 16 rows, three
 // passes over the cache, 302 (and 2 times the memory traffic); in teams of four, 16 warps, 404.
+// Arithmetic on pairs of columns (f32x2): 21 rows 214 -> 206 us, 35 rows 302 -> 299.
 template <int D, int NT>
 struct Shape {
   static constexpr int kTeam = NT <= 2 ? 1 : 2;
@@ -977,9 +978,9 @@ bool make_map(CUtensorMap* map, const uint8_t* base, const Cache& c) {
 }
 
 // Column tiles of 8 query rows an item has: the least that hold a request's rows, at most 5. 64 requests
-// of up to 32768 rows, 4 KV heads, 128 dims: 7 rows with 1, 2, 3 and 5 tiles 130, 155, 208, 282 us; 14
-// rows with 2, 3, 5 167, 216, 292; 21 rows with 3 and 5 224 and 302. 64 dims: 83, 101, 157, 206; 110,
-// 165, 210; 171 and 220.
+// of up to 32768 rows, 4 KV heads, 128 dims: 7 rows with 1, 2, 3 and 5 tiles 128, 155, 202, 280 us; 14
+// rows with 2, 3, 5 167, 210, 290; 21 rows with 3 and 5 220 and 302. 64 dims: 83, 101, 157, 200; 109,
+// 165, 208; 171 and 216.
 int column_tiles(const AttnArgs& a) {
   const long rows = (long)a.max_q * (a.H / a.c.Hkv);
   return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 5;

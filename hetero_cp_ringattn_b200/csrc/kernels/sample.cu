@@ -17,15 +17,16 @@
 // One cluster per row: each CTA holds a contiguous slice of the row in shared memory, so the logits
 // are read from memory once. A histogram over d (bins of 1/32; counts for top-k, counts and weight
 // sums for top-p) gives the bin where the cut falls; the tokens up to it, usually a few dozen, are
-// sent to one CTA, sorted and finished there. More than 512 of them (a large k, a flat row, ties) take
+// sent to one CTA, sorted and finished there. A top-k of up to 256 gets its bin from the threads' maxima
+// instead (129 rows of 151936 tokens, k = 40: 70 us; with a count of every token 83). More than 512 of them (a large k, a flat row, ties) take
 // the general way: histograms of the crossing bin until it is small, or the exact tie, then one pass
 // over the kept tokens.
 //
 // Bound: instructions per token (distance, weight) for many rows, the chain of cluster barriers for
 // one. The weight's polynomial runs on packed pairs. Measured on B200, float32 logits: one row of
 // 128256 tokens 20 us; 129 rows of 151936 (78 MB, 12 us of reading) 102 us with mixed settings, greedy
-// alone 32, temperature alone 62, top-k 40 83, top-k 1000 115, top-p 0.9 over random logits (the
-// general way) 179. One CTA a row that reads the row again in every pass instead of holding it: 289.
+// alone 32, temperature alone 62, top-k 40 70, top-k 1000 119, top-p 0.9 over random logits (the
+// general way) 183. One CTA a row that reads the row again in every pass instead of holding it: 289.
 #include <cooperative_groups.h>
 
 #include <cuda_bf16.h>
@@ -154,7 +155,7 @@ struct __align__(16) Shared {
   u64 warp_a[kWarps], warp_b[kWarps];
   u64 slot[2][kMaxCluster];                      // one value of every CTA, pushed by it
   float fslot[kMaxCluster];
-  int list_n;
+  int list_n, sent;
   u64 found;                                     // results one thread hands to the block
   u64 found_cnt, found_w, found_in_cnt;
   int found_bin;
@@ -231,6 +232,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
       top = max_rn(top, f);
     }
   }
+  const float own = top;
   const float temp = a.temperature.ptr ? a.temperature.ptr[b] : a.temperature.value;
   const int top_k = a.top_k.ptr ? a.top_k.ptr[b] : a.top_k.value;
   const float top_p = a.top_p.ptr ? a.top_p.ptr[b] : a.top_p.value;
@@ -242,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     for (int i = tid; i < kBins; i += kThreads) S.hist[i] = make_uint2(0, 0);
   };
   if (use_k || use_p) clear();
-  if (tid == 0) S.list_n = 0;
+  if (tid == 0) S.list_n = S.sent = 0;
   top = warp_max_rn(top);
   float* wf = reinterpret_cast<float*>(S.warp_a);
   if (lane == 0) wf[warp] = top;
@@ -280,7 +282,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     return;
   }
 
-  // ---------------------------------------------------------------- distances, totals, histogram
   auto add_to_bin = [&](int bin, uint32_t w) {
     uint32_t one = 1;
     if (w) {
@@ -309,26 +310,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     auto one = [&](float v) { return equal(v, top) ? 0.f : min_rn(div_rn(sub_rn(top, v), temp), 64.f); };
     return make_float2(one(l.x), one(l.y));
   };
-  u64 sum = 0;                // without a filter: of the kept weights
-  for (int i = s0 + 2 * lane; i < s1; i += 64) {
-    // (slices start 8 elements aligned and a pair past the end stays inside the slice's memory)
-    float2 d = distance2(*reinterpret_cast<const float2*>(x + i));
-    const bool two = i + 1 < s1;
-    if (!two) d.y = 64.f;
-    *reinterpret_cast<float2*>(x + i) = d;
-    if (use_k) {              // counts alone
-      atomicAdd(&S.hist[bin_of(d.x)].x, 1u);
-      if (two) atomicAdd(&S.hist[bin_of(d.y)].x, 1u);
-      continue;
-    }
-    const uint2 w = weight2(d.x, d.y);
-    if (use_p) {
-      add_to_bin(bin_of(d.x), w.x);
-      if (two) add_to_bin(bin_of(d.y), w.y);
-    } else {
-      sum += u64(w.x >= min_w ? w.x : 0u) + (w.y >= min_w ? w.y : 0u);
-    }
-  }
   auto publish = [&] { cluster.sync(); };
   // this warp's, the lower CTAs' and the cluster's sum of `v`, one value a lane, through slot[which]
   auto sum_over = [&](u64 v, int which, u64& mine, u64& below, u64& total) {
@@ -374,16 +355,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
       below += __shfl_sync(0xffffffffu, inc, 31);
     }
   };
-  u64 mine, below, total;
-  if (!filter) {
-    sum_over(sum, 0, mine, below, total);
-    draw([&](int i) {
-      const uint32_t w = weight(x[i]);
-      return w >= min_w ? w : 0u;
-    }, mine, below, total);
-    return;
-  }
-
   // ---------------------------------------------------------------- the bin of the cut
   // The bin where the cluster's count (or weight) reaches `target` (or top_p of the weight in all the
   // bins, for target 0, which it returns). Every CTA sums
@@ -470,6 +441,109 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
     for (int i = s0 + lane; i < s1; i += 32) add_to_bin(bin_of(x[i]), weight(x[i]));
     publish();
   };
+  // Rank 0: the gathered tokens ordered, cut, and the draw among them.
+  auto finish = [&](int n_all, bool by_k, u64 limit) {
+    int size = 32;
+    while (size < n_all) size <<= 1;
+    u64 v = tid < n_all ? S.all[tid] : kAll;
+    v = sort64(v, size, S.list, tid);
+    const bool here = tid < n_all;
+    const uint32_t w = here ? weight(__uint_as_float(uint32_t(v >> 32))) : 0u;
+    auto scan = [&](u64 val, u64& inc, u64& all) {   // inclusive over the block
+      inc = warp_scan64(val, lane);
+      __syncthreads();
+      if (lane == 31) S.warp_a[warp] = inc;
+      __syncthreads();
+      const u64 o = lane < kWarps ? S.warp_a[lane] : 0;
+      inc += warp_sum64(lane < warp ? o : 0);
+      all = warp_sum64(o);
+    };
+    u64 inc, all;
+    bool keep = here && (!by_k || tid < top_k);
+    scan(keep ? w : 0u, inc, all);
+    if (use_p) keep = keep && inc - w < (by_k ? max(share(all, top_p), u64(1)) : limit);
+    keep = keep && w >= min_w;
+    // kept tokens in vocabulary order, (index, weight)
+    v = sort64(keep ? (u64(uint32_t(v)) << 32) | w : kAll, size, S.list, tid);
+    keep = v != kAll;
+    scan(keep ? uint32_t(v) : 0u, inc, all);
+    const u64 target = share(all, fminf(a.u[b], 0.99999994f));
+    if (keep && inc > target && inc - uint32_t(v) <= target) a.token[b] = (long long)(v >> 32);
+  };
+
+  // ---------------------------------------------------------------- top-k by the threads' maxima
+  // The k-th largest of the threads' maxima bounds the k-th largest token from below, so the bin where
+  // their counts reach k holds the cut or lies behind it: one count a thread instead of one a token, and
+  // only the tokens up to that bin need a distance. Their number is not known ahead (each CTA sends
+  // at most one more than fit); too many of them, or a k the threads cannot bound, take the way below.
+  if (use_k && top_k <= kList / 2) {
+    atomicAdd(&S.hist[bin_of(distance2(make_float2(own, own)).x)].x, 1u);
+    publish();
+    find_bin(false, u64(top_k), 0, 0, false);
+    const int bin = S.found_bin;
+    bool done = false;
+    if (bin >= 0 && bin < kBins - 1) {
+      const float end = float(bin + 1) * (1.f / kPerUnit);
+      // a logit below this is farther than `end`, whatever rounds (no bound outside the normal range)
+      const float reach = end * temp;
+      const float least = by_inverse ? top - reach * 1.000001f - (fabsf(top) + reach) * 1e-6f : ninf;
+      Shared* to = cluster.map_shared_rank(&S, 0);
+      auto send = [&](float l, int i) {
+        if (l < least) return;
+        const float d = distance2(make_float2(l, l)).x;
+        if (!(d < end) || atomicAdd(&S.sent, 1) > kList) return;
+        const int at = atomicAdd(&to->list_n, 1);
+        if (at < kList) to->all[at] = (u64(__float_as_uint(d)) << 32) | uint32_t(lo + i);
+      };
+      for (int i = s0 + 2 * lane; i < s1; i += 64) {
+        const float2 l = *reinterpret_cast<const float2*>(x + i);
+        send(l.x, i);
+        if (i + 1 < s1) send(l.y, i + 1);
+      }
+      publish();
+      const int n_all = to->list_n;
+      cluster.barrier_arrive();          // rank 0's count has been read
+      done = n_all <= kList;
+      if (done && rank == 0) finish(n_all, true, 0);
+      cluster.barrier_wait();
+    }
+    if (done) return;
+    if (tid == 0) S.list_n = 0;
+    clear();
+    __syncthreads();
+  }
+
+  // ---------------------------------------------------------------- distances, totals, histogram
+  u64 sum = 0;                // without a filter: of the kept weights
+  for (int i = s0 + 2 * lane; i < s1; i += 64) {
+    // (slices start 8 elements aligned and a pair past the end stays inside the slice's memory)
+    float2 d = distance2(*reinterpret_cast<const float2*>(x + i));
+    const bool two = i + 1 < s1;
+    if (!two) d.y = 64.f;
+    *reinterpret_cast<float2*>(x + i) = d;
+    if (use_k) {              // counts alone
+      atomicAdd(&S.hist[bin_of(d.x)].x, 1u);
+      if (two) atomicAdd(&S.hist[bin_of(d.y)].x, 1u);
+      continue;
+    }
+    const uint2 w = weight2(d.x, d.y);
+    if (use_p) {
+      add_to_bin(bin_of(d.x), w.x);
+      if (two) add_to_bin(bin_of(d.y), w.y);
+    } else {
+      sum += u64(w.x >= min_w ? w.x : 0u) + (w.y >= min_w ? w.y : 0u);
+    }
+  }
+  u64 mine, below, total;
+  if (!filter) {
+    sum_over(sum, 0, mine, below, total);
+    draw([&](int i) {
+      const uint32_t w = weight(x[i]);
+      return w >= min_w ? w : 0u;
+    }, mine, below, total);
+    return;
+  }
+
   bool by_k = use_k;
   publish();                   // the histograms are complete
   u64 limit = find_bin(!by_k, by_k ? u64(top_k) : 0, 0, 0, !by_k);
@@ -500,35 +574,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a, int s
       send(d.y, i + 1);
     }
     publish();                 // the last access to another CTA's shared memory is behind it
-    if (rank == 0) {
-      const int n_all = S.list_n;
-      int size = 32;
-      while (size < n_all) size <<= 1;
-      u64 v = tid < n_all ? S.all[tid] : kAll;
-      v = sort64(v, size, S.list, tid);
-      const bool here = tid < n_all;
-      const uint32_t w = here ? weight(__uint_as_float(uint32_t(v >> 32))) : 0u;
-      auto scan = [&](u64 val, u64& inc, u64& all) {   // inclusive over the block
-        inc = warp_scan64(val, lane);
-        __syncthreads();
-        if (lane == 31) S.warp_a[warp] = inc;
-        __syncthreads();
-        const u64 o = lane < kWarps ? S.warp_a[lane] : 0;
-        inc += warp_sum64(lane < warp ? o : 0);
-        all = warp_sum64(o);
-      };
-      u64 inc, all;
-      bool keep = here && (!by_k || tid < top_k);
-      scan(keep ? w : 0u, inc, all);
-      if (use_p) keep = keep && inc - w < (by_k ? max(share(all, top_p), u64(1)) : limit);
-      keep = keep && w >= min_w;
-      // kept tokens in vocabulary order, (index, weight)
-      v = sort64(keep ? (u64(uint32_t(v)) << 32) | w : kAll, size, S.list, tid);
-      keep = v != kAll;
-      scan(keep ? uint32_t(v) : 0u, inc, all);
-      const u64 target = share(all, fminf(a.u[b], 0.99999994f));
-      if (keep && inc > target && inc - uint32_t(v) <= target) a.token[b] = (long long)(v >> 32);
-    }
+    if (rank == 0) finish(S.list_n, by_k, limit);
     return;
   }
 

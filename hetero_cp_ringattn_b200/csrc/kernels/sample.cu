@@ -17,10 +17,10 @@
 // One cluster per row: each CTA holds a contiguous slice of the row in shared memory, so the logits
 // are read from memory once. A histogram over d (bins of 1/32; counts for top-k, counts and weight
 // sums for top-p) gives the bin where the cut falls; the tokens up to it, usually a few dozen, are
-// sent to one CTA, sorted and finished there. A top-k of up to 256 gets its bin from the threads' maxima
-// instead (129 rows of 151936 tokens, k = 40: 70 us; with a count of every token 83). More than 512 of them (a large k, a flat row, ties) take
-// the general way: histograms of the crossing bin until it is small, or the exact tie, then one pass
-// over the kept tokens.
+// sent to one CTA, sorted and finished there. A top-k of up to 256 gets its bin from the threads'
+// maxima instead (129 rows of 151936 tokens, k = 40: 70 us; with a count of every token 83). More than
+// 512 of them (a large k, a flat row, ties) take the general way: histograms of the crossing bin until
+// it is small, or the exact tie, then one pass over the kept tokens.
 //
 // Bound: instructions per token (distance, weight) for many rows, the chain of cluster barriers for
 // one. The weight's polynomial runs on packed pairs. Measured on B200, float32 logits: one row of

@@ -507,6 +507,29 @@ def test_sample_equals_the_oracle(dev, kind, vocab):
             assert same(sampling.sample(x, u, *s), sampling.sample(x.cpu(), u.cpu(), *s)), s
 
 
+@pytest.mark.parametrize("kind", ["normal", "ties", "one_thread", "flat", "far", "nan"])
+@pytest.mark.parametrize("vocab", [301, 513, 20481, 151936])
+def test_sample_top_k_sizes(dev, kind, vocab):
+    """k from 1 to past what one CTA orders: ties across the cut, the largest tokens all a fixed stride
+    apart (in one thread's share), rows as good as flat, tokens with weight 0 inside the top k, NaN."""
+    g = torch.Generator(device=dev).manual_seed(vocab + len(kind))
+    x = torch.randn(2, vocab, generator=g, device=dev) * 3
+    if kind == "ties":
+        x = (x * 2).round() / 2
+    elif kind == "one_thread":
+        x[:, ::2048] += 30
+    elif kind == "flat":
+        x *= 1e-4
+    elif kind == "far":
+        x[:, 17:] -= 500
+    elif kind == "nan":
+        x[:, ::3] = float("nan")
+    u = torch.rand(2, generator=g, device=dev)
+    for k in (1, 2, 16, 40, 255, 256, 257, 511, 513):
+        for s in ((1.0, k, 1.0, 0.0), (0.6, k, 0.9, 0.0), (3.0, k, 0.7, 0.01)):
+            assert same(sampling.sample(x, u, *s), sampling.sample(x.cpu(), u.cpu(), *s)), (k, s)
+
+
 def test_sample_large_vocabulary_strides_and_row_settings(dev):
     """The longest rows, rows that do not start on 16 bytes, and a row of settings each."""
     g = torch.Generator(device=dev).manual_seed(0)

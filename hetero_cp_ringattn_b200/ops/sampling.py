@@ -23,6 +23,8 @@ from ..utils import launches
 # Taylor coefficients of 2^g, highest power first: the polynomial of the kernel, operation by operation
 _EXP2 = [math.log(2.0) ** i / math.factorial(i) for i in range(7, -1, -1)]
 _LOG2E = 1.4426950408889634
+# the largest float32 below 1: numbers from 1 on and NaN count as it, as in the kernel
+_U_MAX = 1.0 - 2.0 ** -24
 
 Setting = Union[float, int, torch.Tensor]
 
@@ -30,7 +32,8 @@ Setting = Union[float, int, torch.Tensor]
 def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 1.0, top_k: Setting = 0,
            top_p: Setting = 1.0, min_p: Setting = 0.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """One token id (int64) per row of `logits` [rows, vocab] (float32 or bf16; a GPU row holds at most
-    720896 tokens). `u` float32 [rows] in [0, 1). Each setting is a number or one value per row (float32;
+    720896 tokens). `u` float32 [rows] in [0, 1) (below: 0; from 1 on, or NaN:
+    the largest number below 1). Each setting is a number or one value per row (float32;
     top_k int32). temperature <= 0: the lowest index of the maximum. Off: top_k <= 0, top_p outside (0, 1),
     min_p <= 0. NaN logits count as -inf; a row without any other gives -1."""
     if not logits.is_cuda:
@@ -97,6 +100,7 @@ def _sample_host(logits, u, temperature, top_k, top_p, min_p, out) -> torch.Tens
         kept = torch.zeros_like(w)
         kept[order] = ws
         cum = torch.cumsum(kept, 0)
-        target = _share(int(cum[-1]), min(float(u[b]), 0.99999994))
+        r = float(u[b])
+        target = _share(int(cum[-1]), r if r < _U_MAX else _U_MAX)
         out[b] = int(torch.searchsorted(cum, torch.tensor([target]), right=True))
     return out

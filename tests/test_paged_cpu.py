@@ -186,6 +186,17 @@ def test_sample_edge_rows():
         sampling.sample(logits, u[:3])
 
 
+@pytest.mark.parametrize("u", [1.0 - 2.0 ** -24, 1.0, 2.0, float("nan")])
+def test_sample_largest_uniform_number(u):
+    """The second token's weight 2^31 e^-16.23 = 192 is 1.5 times 2^-24 of the total S: u = 1 - 2^-24, the largest
+    float32 below 1, reaches floor(S - S 2^-24), past the first token; one unit of 2^-24 less does not."""
+    logits = torch.tensor([[0.0, -16.23]])
+    w = sampling.weights(torch.tensor([0.0, 16.23])).tolist()
+    assert w[0] == 2 ** 31 and 130 < w[1] < 250
+    assert sampling.sample(logits, torch.tensor([u])).tolist() == [1]
+    assert sampling.sample(logits, torch.tensor([1.0 - 2.0 ** -23])).tolist() == [0]
+
+
 def test_weights_follow_exp():
     d = torch.linspace(0, 20, 4001)
     w = sampling.weights(d).double() / 2.0 ** 31

@@ -546,6 +546,17 @@ def test_sample_large_vocabulary_strides_and_row_settings(dev):
     assert same(sampling.sample(x, u, t, k, p, m), sampling.sample(x.cpu(), u.cpu(), t.cpu(), k.cpu(), p.cpu(), m.cpu()))
 
 
+@pytest.mark.parametrize("u", [1.0 - 2.0 ** -24, 1.0 - 2.0 ** -23, 1.0, float("nan"), -0.5])
+def test_sample_ends_of_the_uniform_range(dev, u):
+    """Every row drawn at the end of its range: the last kept tokens' weights decide."""
+    g = torch.Generator(device=dev).manual_seed(11)
+    x = torch.randn(300, 2000, generator=g, device=dev) * 4
+    x[0, 1:], x[0, 1] = float("-inf"), x[0, 0] - 16.23
+    v = torch.full((300,), u, device=dev)
+    for s in ((1.0, 0, 1.0, 0.0), (0.8, 50, 0.95, 0.0)):
+        assert same(sampling.sample(x, v, *s), sampling.sample(x.cpu(), v.cpu(), *s))
+
+
 def test_sample_frequencies(dev):
     """200,000 draws from one row: every token's count within 5 standard deviations of its share
     (64 tokens: a chance of 4e-5 that any is outside)."""

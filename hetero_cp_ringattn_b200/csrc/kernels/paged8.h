@@ -88,7 +88,8 @@ struct AttnArgs {
   const int* table;      // [B][width]
   const int* kv_len;     // [B]
   const int* cu;         // [B + 1] or null (one token a row)
-  int B, T, H, width, max_q;
+  int B, T, H, width;
+  int max_q;             // a request's most query tokens, for the choice of shapes (more are right, but slower)
   float scale;
   void* o;               // [T][H][D]
   float* lse;            // [H][T] or null

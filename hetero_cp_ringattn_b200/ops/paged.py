@@ -111,11 +111,13 @@ def attention_kv8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: to
     """Attention of q [tokens, heads, D] (bf16 or f16) over the requests' cached rows.
 
     Request b has the query tokens cu[b] .. cu[b + 1] - 1 (None: token b) and kv_len[b] cached rows; its
-    query token i of m sees rows 0 .. kv_len[b] - m + i. `max_q` bounds m. Returns (o [tokens, heads, D],
-    lse [heads, tokens] natural log, or None); a token that sees no row gets o = 0, lse = -inf, so the
-    partials of several ranks' shards merge like the other attention's (`reference.merge_partials`). At
-    most 1024 requests a call. Meant for decode steps and short segments (drafts to verify): for a long
-    segment read the rows back with `gather_kv8` and use `kernels.attention`."""
+    query token i of m sees rows 0 .. kv_len[b] - m + i. `max_q` is the most query tokens that a request
+    has: the tiles' shape goes by it, the results do not (a request with more is right, but slower). `cu`
+    past the tokens of q is reported to `status`. Returns (o [tokens, heads, D], lse [heads, tokens] natural
+    log, or None); a token that sees no row gets o = 0, lse = -inf, so the partials of several ranks' shards
+    merge like the other attention's (`reference.merge_partials`). At most 1024 requests a call. Meant for
+    decode steps and short segments (drafts to verify): for a long segment read the rows back with
+    `gather_kv8` and use `kernels.attention`."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     if not q.is_cuda:

@@ -294,6 +294,41 @@ def test_attention_ragged_query_tokens(dev, code, heads, hkv, dim, page, most):
     check_attention(q, *_cache(lens, page, hkv, dim, code, dev, seed=most), lens, cu)
 
 
+@pytest.mark.parametrize("max_q", [1, 2, 3])
+@pytest.mark.parametrize("heads,hkv,dim", [(8, 2, 128), (4, 4, 64)])
+def test_attention_results_do_not_depend_on_max_q(dev, heads, hkv, dim, max_q):
+    """Requests with more query tokens than max_q says (it defaults to 1): the causal limits, and every
+    query row of a request that many CTAs share."""
+    lens, qn = [9, 3000, 40, 6, 2500], [5, 5, 0, 9, 33]
+    cu = [0]
+    for n in qn:
+        cu.append(cu[-1] + n)
+    q = torch.randn(cu[-1], heads, dim, device=dev).bfloat16()
+    k, v, ks, vs, table = _cache(lens, 32, hkv, dim, "e4m3", dev)
+    kv_len, cut = (torch.tensor(x, dtype=torch.int32, device=dev) for x in (lens, cu))
+    want, want_l = check_attention(q, k, v, ks, vs, table, lens, cu)
+    st = status_tensor(dev)
+    kw = {} if max_q == 1 else dict(max_q=max_q)
+    got, got_l = paged.attention_kv8(q, k, v, ks, vs, table, kv_len, cut, status=st, **kw)
+    assert int(st[0]) == 0
+    assert torch.equal(torch.isinf(got_l), torch.isinf(want_l))
+    # each call's o is within one rounding of the exact value and 2^-10 of sum p |v| (at most max |v|)
+    top = float((_abs(v).float().nan_to_num(0.0).clamp(max=400.0) * vs.view(*vs.shape, 1, 1)).max())
+    assert ((got.float() - want.float()).abs() <= 2 * (2.0 ** -8 * want.float().abs() + 2.0 ** -10 * top)).all()
+    assert ((got_l - want_l)[torch.isfinite(want_l)].abs() <= 1e-4).all()
+
+
+def test_attention_query_offsets_past_the_tokens_are_reported(dev):
+    lens = [40, 50]
+    k, v, ks, vs, table = _cache(lens, 16, 1, 64, "e4m3", dev)
+    q = torch.randn(3, 2, 64, device=dev).bfloat16()
+    for cu, bad in (([0, 2, 3], False), ([0, 2, 5], True), ([-1, 2, 3], True), ([0, 2, 1], True)):
+        st = status_tensor(dev)
+        o, _ = paged.attention_kv8(q, k, v, ks, vs, table, torch.tensor(lens, dtype=torch.int32, device=dev),
+                                   torch.tensor(cu, dtype=torch.int32, device=dev), max_q=3, status=st)
+        assert (int(st[0]) == 18) == bad and torch.isfinite(o).all()
+
+
 @pytest.mark.parametrize("batch,longest", [(1, 20011), (3, 9000), (40, 700), (300, 90), (1024, 40)])
 def test_attention_work_split(dev, batch, longest):
     """One long request (every CTA on the same heads) to more requests than CTAs."""

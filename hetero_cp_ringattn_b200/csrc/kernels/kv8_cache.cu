@@ -58,7 +58,14 @@ __device__ __forceinline__ void rope_q(const AppendArgs& a, uint32_t item) {
   if (t >= a.T) return;
   const int pos = a.pos[t];
   const bool ok = pos >= 0 && pos < a.max_pos;
-  if (!ok && chunk == 0 && h0 == 0) report_error(a.status, int(StatusCode::kOutOfBounds), 401, pos, t);
+  if (!ok) {   // q of a token without a place is 0
+    if (chunk == 0 && h0 == 0) report_error(a.status, int(StatusCode::kOutOfBounds), 401, pos, t);
+    for (int h = h0; h < min(a.H, h0 + kQHeads); ++h) {
+      uint4* o = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.q_out) + ((long)t * a.H + h) * D + chunk * 8);
+      o[0] = o[D / 16] = make_uint4(0, 0, 0, 0);
+    }
+    return;
+  }
   float c[8], s[8];
 #pragma unroll
   for (int g = 0; g < kQHeads; g += kAtOnce) {
@@ -69,7 +76,7 @@ __device__ __forceinline__ void rope_q(const AppendArgs& a, uint32_t item) {
       r1[i] = load_raw8<DT>(a.x, at);
       r2[i] = load_raw8<DT>(a.x, at + D / 2);
     }
-    if (g == 0) load_cos_sin(a, ok ? pos : 0, chunk * 8, c, s);
+    if (g == 0) load_cos_sin(a, pos, chunk * 8, c, s);
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
       const int h = h0 + g + i;
@@ -87,7 +94,7 @@ __device__ __forceinline__ void rope_q(const AppendArgs& a, uint32_t item) {
   }
 }
 
-// A unit's place: checked before anything is addressed by it.
+// A unit's place: checked before anything is addressed by it, its positions against the rotary table too.
 struct UnitAt {
   int t0, n, p0, start;   // first token, tokens, first position, first offset in the block
   int page;               // -1: nothing to do
@@ -103,7 +110,8 @@ __device__ __forceinline__ UnitAt unit_at(const AppendArgs& a, uint32_t ui, bool
   z.n = u.z;
   z.p0 = u.w;
   z.start = u.w - block * P;
-  const bool ok = u.x < a.R && u.y >= 0 && u.z >= 1 && u.z <= a.T - u.y && u.w >= 0 && z.start + u.z <= P && block < a.width;
+  const bool ok = u.x < a.R && u.y >= 0 && u.z >= 1 && u.z <= a.T - u.y && u.w >= 0 && z.start + u.z <= P && block < a.width &&
+                  u.z <= a.max_pos - u.w;
   const int page = ok ? a.table[(long)u.x * a.width + block] : -1;
   if (page >= 0 && page < a.c.pages) z.page = page;
   else if (report) report_error(a.status, int(StatusCode::kOutOfBounds), 402, page, int(ui));
@@ -119,7 +127,7 @@ __device__ __forceinline__ void unit_values(const AppendArgs& a, int t, int pos,
   load8<DT>(a.x, at + D / 2, x2);
   if (rotate) {
     float c[8], s[8];
-    load_cos_sin(a, min(pos, a.max_pos - 1), chunk * 8, c, s);
+    load_cos_sin(a, pos, chunk * 8, c, s);
     rotate8(x1, x2, c, s);
   }
 }
@@ -241,7 +249,7 @@ __device__ __forceinline__ void store_block(const AppendArgs& a, uint32_t cta, i
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
     const int item = k * team + me, i = item / kChunks, chunk = item % kChunks;
-    if (!kv && i < n) load_cos_sin(a, min(z.p0 + i, a.max_pos - 1), chunk * 8, c[k], s[k]);
+    if (!kv && i < n) load_cos_sin(a, z.p0 + i, chunk * 8, c[k], s[k]);
   }
   for (int h = h0; h < h0 + heads; ++h) {     // (every team of the CTA makes all turns: barriers)
     const bool some = n > 0 && h < h1;

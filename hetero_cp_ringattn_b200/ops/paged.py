@@ -94,8 +94,9 @@ def rope_append_kv8(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos
     `qkv` [tokens, (heads + 2 kv_heads) * D] in float32, bf16 or f16; `pos`, `unit` of the step's plan
     (`plan_step`, or the same lists made elsewhere). Block scales: a new block's follows from its new
     tokens, an open block's grows with them (its stored codes are rescaled). Returns q [tokens, heads, D]
-    in `q_out`'s type (default: qkv's, bf16 for float32). `status`: int32 [>= 4] error word for
-    positions and page ids out of range (the access is skipped)."""
+    in `q_out`'s type (default: qkv's, bf16 for float32). A token whose position lies outside the rotary
+    tables gets q = 0, and a unit whose row, tokens, positions or page id are out of range stores nothing;
+    both are reported to `status`, an int32 [>= 4] error word (on the CPU they raise and nothing is written)."""
     if not qkv.is_cuda:
         return pref.rope_append_kv8(qkv, cos, sin, pos, unit, block_table, k, v, k_scale, v_scale, heads, q_out)
     q = native().rope_append_kv8(qkv, cos, sin, pos, unit, block_table, k, v, k_scale, v_scale, heads, q_out, status)

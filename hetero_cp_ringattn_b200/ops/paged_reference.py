@@ -106,11 +106,25 @@ def _store(x, unit, block_table, data, scale) -> None:
         data[page, :, start:start + m] = encode(new / s.view(1, -1, 1), code).transpose(0, 1)
 
 
+def _check_places(unit, block_table, pages: int, P: int, tokens: int, pos, positions: int) -> None:
+    """Raise for what the kernel reports to its status word, before anything is written."""
+    if tokens and not 0 <= int(pos.min()) <= int(pos.max()) < positions:
+        raise RingError(f"a position outside the rotary tables' {positions}")
+    rows, width = block_table.shape
+    for r, t0, m, p0 in unit.tolist():
+        if r < 0:
+            continue
+        ok = r < rows and t0 >= 0 and 1 <= m <= tokens - t0 and p0 >= 0 and p0 % P + m <= P and p0 // P < width
+        if not ok or p0 + m > positions or not 0 <= int(block_table[r, p0 // P]) < pages:
+            raise RingError(f"unit {(r, t0, m, p0)} is out of range")
+
+
 def rope_append_kv8(qkv, cos, sin, pos, unit, block_table, k, v, k_scale, v_scale, heads: int,
                     q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
     T, Hkv, D = qkv.shape[0], k.shape[1], k.shape[3]
     if qkv.shape[1] != (heads + 2 * Hkv) * D:
         raise RingError("qkv must have heads + 2 kv_heads heads a row")
+    _check_places(unit, block_table, k.shape[0], k.shape[2], T, pos[:T], cos.shape[0])
     x = qkv.float().view(T, heads + 2 * Hkv, D)
     c, s = cos[pos[:T].long()].unsqueeze(1), sin[pos[:T].long()].unsqueeze(1)
     x1, x2 = x[:, :heads + Hkv, : D // 2], x[:, :heads + Hkv, D // 2:]

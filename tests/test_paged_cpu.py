@@ -124,6 +124,23 @@ def test_append_values_are_within_a_code_step(code):
         assert ((got - want).abs() <= step * 1.0001).all()
 
 
+@pytest.mark.parametrize("unit,table,pos", [
+    ([0, 0, 2, 7], [1], [7, 8]), ([0, 0, 2, 7], [1], [6, 7]), ([0, 0, 2, 0], [1], [-1, 0]), ([0, 0, 2, -1], [1], [0, 1]),
+    ([0, 0, 2, 0], [-1], [0, 1]), ([0, 0, 2, 0], [2], [0, 1]), ([1, 0, 2, 0], [1], [0, 1]), ([0, 1, 2, 0], [1], [0, 1]),
+    ([0, 0, 2, 16], [1], [0, 1])])
+def test_append_refuses_places_out_of_range(unit, table, pos):
+    """Positions past and before the rotary tables (of 8 positions, pages of 16), page ids, rows and tokens
+    that are not there: refused, with nothing written."""
+    c = Kv8Cache(1, 1, 64, rows=1, max_context=16, page=16, pages=2)
+    cos, sin = ref.rope_cos_sin(torch.arange(8), 64, 10000.0)
+    i32 = dict(dtype=torch.int32)
+    with pytest.raises(RingError):
+        paged.rope_append_kv8(torch.randn(2, 3 * 64), cos, sin, torch.tensor(pos, **i32), torch.tensor([unit], **i32),
+                              torch.tensor([table], **i32), *c.layer(0), heads=1)
+    assert not c.k.view(torch.uint8).any() and not c.v.view(torch.uint8).any()
+    assert (c.k_scale == 1).all() and (c.v_scale == 1).all()
+
+
 def test_scale_is_the_smallest_power_of_two_that_holds_the_maximum():
     for code, top in ((torch.float8_e4m3fn, 448.0), (torch.int8, 127.0)):
         a = torch.cat([torch.tensor([top, top * 1.0001, top * 0.5, 1e-30, 0.0, 1e30]), torch.rand(1000) * 1000])

@@ -172,6 +172,34 @@ def test_append_reports_and_skips_bad_places(dev):
         assert int(st[0]) == 18 and torch.equal(k.view(torch.uint8), before)
 
 
+@pytest.mark.parametrize("n,page", [(2, 16), (16, 16), (33, 64)])
+@pytest.mark.parametrize("shift", [-1, 1])
+def test_append_writes_nothing_past_the_rotary_tables(dev, n, page, shift):
+    """Row 0's positions leave the tables (at their end by one, or below 0), row 1's are good: row 0's codes,
+    scales and neighbours stay, its q is 0 where the position is bad, and row 1 is as alone. Units of 2
+    tokens take the short form, those of 16 and more the block form."""
+    tab = page // 2 + n
+    p0 = page // 2 + 1 if shift > 0 else -1
+    if shift > 0 and p0 % page + n > page:
+        p0, tab = page, page + n - 1                    # a whole block that ends one past the tables
+    k, v, ks, vs = _strided_cache(4, 2, page, 64, "e4m3", dev)
+    cos, sin = (t.to(dev) for t in ref.rope_cos_sin(torch.arange(tab), 64, 10000.0))
+    x = torch.randn(2 * n, (2 + 4) * 64, device=dev)
+    pos = torch.cat([torch.arange(p0, p0 + n), torch.arange(n)]).to(torch.int32).to(dev)
+    unit = torch.tensor([[0, 0, n, p0], [1, n, n, 0]], dtype=torch.int32, device=dev)
+    table = torch.tensor([[3, 1], [2, 0]], dtype=torch.int32, device=dev)
+    want = [t.clone() for t in (k, v, ks, vs)]
+    want_q = paged.rope_append_kv8(x[n:], cos, sin, pos[n:], unit[1:] - torch.tensor([0, n, 0, 0], device=dev, dtype=torch.int32),
+                                   table, *want, heads=2)
+    st = status_tensor(dev)
+    q = paged.rope_append_kv8(x, cos, sin, pos, unit, table, k, v, ks, vs, heads=2, status=st)
+    assert int(st[0]) == 18
+    for a, b in zip((k, v, ks, vs), want):
+        assert same(a, b.cpu())
+    bad = (pos < 0) | (pos >= tab)
+    assert bad.any() and (q[bad] == 0).all() and (q[:n][~bad[:n]] != 0).any() and torch.equal(q[n:], want_q)
+
+
 def test_append_refusals(dev):
     k, v, ks, vs = _strided_cache(2, 1, 16, 64, "e4m3", dev)
     cos, sin = (t.to(dev) for t in ref.rope_cos_sin(torch.arange(16), 64, 10000.0))

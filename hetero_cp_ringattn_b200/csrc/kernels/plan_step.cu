@@ -4,7 +4,8 @@
 //   need_r = ceil((old_r + n_r) / P) - ceil(old_r / P)    pages taken from the FIFO ring, in row order
 //   slot(t) = table[r][p / P] * P + p % P                 for the token at position p of row r
 // and a "unit" per block that the new tokens touch, the work list of the append. A step that does
-// not fit (tokens, table width or free pages) changes nothing and says so in info[3].
+// not fit (tokens, table width, free pages, or more pages given back than the ring has places for)
+// changes nothing and says so in info[3].
 //
 // Bound: latency. The arrays are a few bytes per row and token, so one launch does the whole step:
 // every CTA scans all rows (four sums at once) and the CTAs share the tokens, units and pages to
@@ -131,6 +132,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(PlanArgs a) {
   if (total.n > a.max_tokens) status = 3;
   else if (any_wide) status = 2;
   else if (total.need > avail + total.back) status = 1;
+  else if (avail + total.back > a.ring_size) status = 4;   // (the writes to the ring below rely on it)
   const bool ok = status == 0;
   if (!ok) total = Sums{0, 0, 0, 0};
   for (int r = r0; r < r1; ++r) {

@@ -55,7 +55,8 @@ class StepPlan:
                    info=torch.empty(4, **i32))
 
 
-PLAN_STATUS = {0: "ok", 1: "not enough free pages", 2: "a row outgrows its block table", 3: "more tokens than the plan holds"}
+PLAN_STATUS = {0: "ok", 1: "not enough free pages", 2: "a row outgrows its block table", 3: "more tokens than the plan holds",
+               4: "more pages given back than the ring has places for"}
 
 
 def max_units(rows: int, page: int, max_tokens: int) -> int:
@@ -70,7 +71,8 @@ def plan_step(add: torch.Tensor, kv_len: torch.Tensor, block_table: torch.Tensor
     `kv_len` int32 [rows] lengths; `block_table` int32 [rows, width]; `ring` int32 [pages], a FIFO of
     free page ids whose entries counters[0] .. counters[1] - 1 (int64, modulo the ring's size) are free.
     New pages are taken in row order, first from the ring, then from rows released in this same step;
-    released pages join the ring's end in row order. `block_table` and `ring` are updated in place (new
+    released pages join the ring's end in row order (the free and the released pages of a step together must
+    not exceed the ring's size: it holds every page of the pool). `block_table` and `ring` are updated in place (new
     entries only), the new lengths and counters go to the plan. A step that does not fit changes nothing
     and sets info[3] (PLAN_STATUS). At most 4096 rows."""
     if out is None:

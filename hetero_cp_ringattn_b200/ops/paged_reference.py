@@ -47,6 +47,8 @@ def plan_step(add, kv_len, block_table, ring, counters, page: int, max_tokens: i
         status = 2
     elif sum(need) > min(max(tail - head, 0), size) + sum(back):
         status = 1
+    elif min(max(tail - head, 0), size) + sum(back) > size:
+        status = 4
     out.row.fill_(-1)
     out.pos.zero_()
     out.slot.fill_(-1)

@@ -75,6 +75,28 @@ def test_plan_refuses_what_does_not_fit(add, status):
         assert p.kv_len.tolist() == [24, 0, 0] and table[0].tolist() == [3, 2, 0, -1] and p.counters.tolist() == [7, 8]
 
 
+def _crowded_ring(free):
+    """Row 0 holds 3 pages, row 1 one, and the ring has 4 places, `free` of them taken: releasing row 0 fits
+    up to one free page."""
+    kv_len = torch.tensor([40, 16], dtype=torch.int32)
+    table = torch.tensor([[5, 6, 7], [8, -1, -1]], dtype=torch.int32)
+    return kv_len, table, torch.tensor([0, 1, 2, 3], dtype=torch.int32), torch.tensor([7, 7 + free])
+
+
+@pytest.mark.parametrize("free,status", [(0, 0), (1, 0), (2, 4), (4, 4), (9, 4)])
+def test_plan_gives_back_no_more_pages_than_the_ring_holds(free, status):
+    kv_len, table, ring, counters = _crowded_ring(free)
+    p = paged.plan_step(torch.tensor([-1, 0], dtype=torch.int32), kv_len, table, ring, counters, page=16, max_tokens=4)
+    assert int(p.info[3]) == status and status in paged.PLAN_STATUS
+    if status:
+        assert ring.tolist() == [0, 1, 2, 3] and p.kv_len.tolist() == [40, 16] and p.counters.tolist() == [7, 7 + free]
+    else:
+        want = [0, 1, 2, 3]
+        for i, page_id in enumerate((5, 6, 7)):
+            want[(7 + free + i) % 4] = page_id
+        assert ring.tolist() == want and p.kv_len.tolist() == [0, 16] and p.counters.tolist() == [7, 10 + free]
+
+
 def test_cache_mirror_and_capacity_errors():
     c = Kv8Cache(1, 2, 64, rows=2, max_context=100, page=16, pages=6)
     c.plan(torch.tensor(c.reserve([50, 17]), dtype=torch.int32), 67)

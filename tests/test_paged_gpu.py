@@ -71,6 +71,25 @@ def test_plan_equals_the_oracle(dev, rows, width, page, room, kind, in_place):
     assert int(got.info[3]) == {"toomany": 3, "wide": 2, "nopages": 1}.get(kind, 0)
 
 
+@pytest.mark.parametrize("free", [0, 1, 2, 4, 9])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_plan_gives_back_no_more_pages_than_the_ring_holds(dev, free, in_place):
+    from test_paged_cpu import _crowded_ring
+    add = torch.tensor([-1, 3], dtype=torch.int32)
+    host = _crowded_ring(free)
+    gpu = [t.to(dev) for t in host]
+    # the ring lies inside a longer tensor: what stands behind it must stay
+    wide = torch.full((64,), -7, dtype=torch.int32, device=dev)
+    wide[:4] = gpu[2]
+    gpu[2] = wide[:4]
+    want = paged.plan_step(add, *host, page=16, max_tokens=8)
+    out = paged.StepPlan.empty(2, 16, 8, dev, kv_len=gpu[0] if in_place else None, counters=gpu[3] if in_place else None)
+    got = paged.plan_step(add.to(dev), *gpu, page=16, max_tokens=8, out=out)
+    for name in ("cu", "row", "pos", "slot", "unit", "kv_len", "counters", "info"):
+        assert same(getattr(got, name), getattr(want, name)), name
+    assert same(gpu[1], host[1]) and same(gpu[2], host[2]) and (wide[4:] == -7).all()
+
+
 def test_plan_refusals(dev):
     kv_len, table, ring, counters = (x.to(dev) for x in _plan_state(4, 3, 16, 20, 0))
     add = torch.ones(4, dtype=torch.int32, device=dev)

@@ -428,9 +428,22 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
   int spent = 0, spent_at = 0, spent_tile = 0;   // team: stages that take copies at the next step
   long long x = x0;
   // A wait that ran out (reported) ends the waiting and the copies, not the loop: the barriers that two
-  // warps share stay matched, and the rest of the range is computed on whatever the ring holds.
+  // warps share stay matched, and the rest of the range is computed on whatever the ring holds. No other
+  // report ends it: a bad page id of one request (or a word that an earlier call left set) says nothing
+  // about this stream's copies, which land in this CTA's memory and have to be waited for.
   bool alive = true;
   auto stage_at = [&](int i) { return stage + i >= kStages ? stage + i - kStages : stage + i; };
+  auto parity_at = [&](int i) { return stage + i >= kStages ? phase ^ 1 : phase; };
+  auto await = [&](int q) {
+    if (mbar_wait(&bars[stream][stage_at(q)], parity_at(q), nullptr, 0)) return;
+    report_error(a.status, int(StatusCode::kMbarTimeout), 412, int(x - x0));
+    alive = false;
+    // the copies still in flight, together as long again (the ring holds the tiles from x on, without the
+    // stages that have not taken a new copy yet)
+    const uint64_t t0 = globaltimer_ns();
+    for (int i = q + 1; i < kStages - spent && x + i < x1; ++i)
+      while (!mbar_try_wait(smem_u32(&bars[stream][stage_at(i)]), parity_at(i)) && globaltimer_ns() - t0 < kPipeTimeoutNs) {}
+  };
   while (x < x1) {
     const Place p = place_of(x);
     const int n = p.n, qn = p.qn;
@@ -507,7 +520,7 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
       const int count = min(kStep, end - tile);           // tiles of this step
 #pragma unroll
       for (int q = 0; q < kStep; ++q)
-        if (alive && q < count) alive = mbar_wait(&bars[stream][stage_at(q)], stage + q >= kStages ? phase ^ 1 : phase, a.status, 412);
+        if (alive && q < count) await(q);
       const int base = tile * kTile;
       const uint32_t ring_at = smem_u32(ring);
       const bool edge = base + kStep * kTile > least || count < kStep;

@@ -456,6 +456,29 @@ def test_attention_page_ids_out_of_range_are_reported(dev):
         assert int(st[0]) == 18 and int(st[2]) == bad and torch.isfinite(o).all()
 
 
+def test_attention_of_other_requests_does_not_depend_on_a_report(dev):
+    """A status word that is set already, and a bad page id of one request, leave the others' outputs as
+    they are (and the first report stands)."""
+    lens = [3000, 20000, 700, 5000]
+    k, v, ks, vs, table = _cache(lens, 16, 2, 128, "e4m3", dev, garbage=False)
+    kv_len = torch.tensor(lens, dtype=torch.int32, device=dev)
+    for heads, most in ((8, 1), (16, 3)):
+        cu = torch.arange(0, 4 * most + 1, most, dtype=torch.int32, device=dev)
+        q = torch.randn(4 * most, heads, 128, device=dev).bfloat16()
+        want, want_l = paged.attention_kv8(q, k, v, ks, vs, table, kv_len, cu, max_q=most)
+        st = status_tensor(dev)
+        st[0] = 99
+        got, got_l = paged.attention_kv8(q, k, v, ks, vs, table, kv_len, cu, max_q=most, status=st)
+        assert torch.equal(got, want) and torch.equal(got_l, want_l) and st.tolist() == [99] + [0] * 7
+        bad = table.clone()
+        bad[1, ::7] = -1
+        st = status_tensor(dev)
+        got, got_l = paged.attention_kv8(q, k, v, ks, vs, bad, kv_len, cu, max_q=most, status=st)
+        assert int(st[0]) == 18 and int(st[1]) == 411
+        rows = [t for t in range(4 * most) if t // most != 1]
+        assert torch.equal(got[rows], want[rows]) and torch.equal(got_l[:, rows], want_l[:, rows])
+
+
 def test_attention_lengths_past_the_table_are_cut(dev):
     k, v, ks, vs, table = _cache([64], 16, 1, 64, "e4m3", dev)
     q = torch.randn(1, 2, 64, device=dev).bfloat16()

@@ -42,6 +42,8 @@ hcp::kv8::Cache cache_of(const Tensor& k, const Tensor& v, const Tensor& ks, con
   TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes() && k.strides() == v.strides() && k.scalar_type() == v.scalar_type(),
               "k and v must be [pages, kv_heads, page, head_dim] of one type, shape and strides");
   TORCH_CHECK(k.scalar_type() == torch::kFloat8_e4m3fn || k.scalar_type() == torch::kInt8, "the cache holds float8_e4m3fn or int8");
+  // (before anything divides by the head count)
+  TORCH_CHECK(k.numel() > 0, "the cache must have a page, a KV head, tokens and dims");
   TORCH_CHECK(k.stride(3) == 1, "cache rows must be contiguous");
   TORCH_CHECK(ks.dim() == 2 && ks.size(0) == k.size(0) && ks.size(1) == k.size(1) && ks.sizes() == vs.sizes() &&
                   ks.strides() == vs.strides() && ks.scalar_type() == torch::kFloat32 && vs.scalar_type() == torch::kFloat32,

@@ -564,6 +564,22 @@ def test_attention_and_gather_refusals(dev):
     assert o.shape == (0, 4, 64)
 
 
+@pytest.mark.parametrize("shape", [(2, 0, 16, 64), (0, 1, 16, 64), (2, 1, 0, 64), (2, 1, 16, 0)])
+def test_empty_caches_are_refused(dev, shape):
+    k, v = (torch.zeros(shape, dtype=torch.int8, device=dev) for _ in "kv")
+    ks, vs = (torch.ones(shape[:2], device=dev) for _ in "kv")
+    table, n = torch.zeros(1, 1, dtype=torch.int32, device=dev), torch.ones(1, dtype=torch.int32, device=dev)
+    q = torch.zeros(1, 4, shape[3], dtype=torch.bfloat16, device=dev)
+    with pytest.raises(RuntimeError, match="the cache must have"):
+        paged.attention_kv8(q, k, v, ks, vs, table, n, scale=1.0)
+    with pytest.raises(RuntimeError, match="the cache must have"):
+        paged.gather_kv8(k, v, ks, vs, table[0], 1)
+    tab = torch.zeros(4, shape[3] // 2, device=dev)
+    with pytest.raises(RuntimeError, match="the cache must have"):
+        paged.rope_append_kv8(torch.zeros(1, (4 + 2 * shape[1]) * shape[3], device=dev), tab, tab, n,
+                              torch.zeros(1, 4, dtype=torch.int32, device=dev), table, k, v, ks, vs, heads=4)
+
+
 # --------------------------------------------------------------------------- gather
 @pytest.mark.parametrize("code,page,hkv,dim,n", [("e4m3", 16, 1, 64, 1), ("int8", 64, 3, 128, 200), ("e4m3", 128, 8, 64, 1000),
                                                  ("int8", 32, 2, 64, 33), ("e4m3", 64, 2, 128, 0)])

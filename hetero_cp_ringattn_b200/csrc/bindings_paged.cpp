@@ -94,8 +94,8 @@ void plan_step(const Tensor& add, const Tensor& kv_len, const Tensor& table, con
   TORCH_CHECK(unit.size(1) == 4, "unit must be [units, 4]");
   TORCH_CHECK(counters.size(0) == 2 && counters_out.size(0) == 2 && info.size(0) == 4, "counters must have 2 entries, info 4");
   TORCH_CHECK(page >= 1 && page <= (1 << 20), "page must be 1 to 2^20 tokens");
-  TORCH_CHECK(R <= hcp::kv8::kPlanMaxRows && T < (1ll << 31) && table.size(1) < (1ll << 31) && ring.size(0) < (1ll << 31),
-              "plan_step: at most ", std::to_string(hcp::kv8::kPlanMaxRows), " rows, and every size below 2^31");
+  TORCH_CHECK(R <= hcp::kv8::kPlanMaxRows && T < (1ll << 30) && unit.size(0) < (1ll << 30) && table.size(1) < (1ll << 31) && ring.size(0) < (1ll << 31),
+              "plan_step: at most ", std::to_string(hcp::kv8::kPlanMaxRows), " rows, fewer than 2^30 tokens and units, and every other size below 2^31");
   TORCH_CHECK(unit.size(0) >= std::min(T, T / page + 2 * R), "unit must have min(tokens, tokens / page + 2 rows) entries");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(row.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(pos.data_ptr()) % 16 == 0 &&
                   reinterpret_cast<uintptr_t>(slot.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(unit.data_ptr()) % 16 == 0,
@@ -179,7 +179,8 @@ std::tuple<Tensor, Tensor> gather_kv8(const Tensor& k, const Tensor& v, const Te
   a.c = cache_of(k, v, ks, vs);
   const auto dev = k.device();
   check_array(table, "block_table row", torch::kInt32, 1, dev);
-  TORCH_CHECK(n >= 0 && n < (1ll << 31), "rows to gather out of range");
+  // (the kernel numbers a head's 16-byte pieces in 32 bits; before any buffer is made)
+  TORCH_CHECK(n >= 0 && n * a.c.D < (1ll << 35) - (1ll << 12), "gather_kv8: rows to gather out of range");
   const c10::cuda::CUDAGuard g(dev);
   TORCH_CHECK(k_buf.has_value() == v_buf.has_value(), "give both output buffers or none");
   Tensor k_out, v_out;

@@ -413,6 +413,7 @@ const char* gather(const GatherArgs& a, cudaStream_t s) {
   if (a.n < 1) return nullptr;
   if ((a.n + a.c.P - 1) / a.c.P > a.width) return "gather_kv8: more rows than the table holds";
   if (a.c.Hkv > 65535) return "gather_kv8: too many heads";
+  if ((long)a.n * (a.c.D / 16) >= (1l << 31) - kThreads) return "gather_kv8: too many rows";   // (32-bit piece numbers)
   cudaError_t e = a.c.D == 64 ? (a.c.code == kInt8 ? launch_gather<64, true>(a, s) : launch_gather<64, false>(a, s))
                               : (a.c.code == kInt8 ? launch_gather<128, true>(a, s) : launch_gather<128, false>(a, s));
   return e == cudaSuccess ? nullptr : cudaGetErrorString(e);

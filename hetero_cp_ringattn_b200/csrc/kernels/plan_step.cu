@@ -290,6 +290,7 @@ const char* plan_step(const PlanArgs& args, cudaStream_t s) {
   if ((long long)a.R * a.width >= (1ll << 31) || (long long)a.width * a.P >= (1ll << 30))
     return "plan_step: table too large";
   if (a.max_tokens < 1 || a.max_units < 1) return "plan_step: max_tokens and max_units must be positive";
+  if (a.max_tokens >= (1 << 30)) return "plan_step: fewer than 2^30 tokens";   // (32-bit token numbers, rounded up to fours)
   // threads for the rows and the token quads of a small step; CTAs for the writes of a large one
   const int quads = (a.max_tokens + 3) / 4;
   const int work = quads > a.max_units ? quads : a.max_units;

@@ -580,6 +580,24 @@ def test_empty_caches_are_refused(dev, shape):
                               torch.zeros(1, 4, dtype=torch.int32, device=dev), table, k, v, ks, vs, heads=4)
 
 
+def test_sizes_past_32_bit_numbers_are_refused(dev):
+    """A gather of 2^28 rows of 128 dims (2^31 pieces of 16 bytes), and a plan of 2^30 tokens: refused before
+    anything of that size is allocated or launched."""
+    k, v = (torch.zeros(1, 1, 128, 128, dtype=torch.int8, device=dev) for _ in "kv")
+    ks, vs = (torch.ones(1, 1, device=dev) for _ in "kv")
+    with pytest.raises(RuntimeError, match="rows to gather out of range"):
+        paged.gather_kv8(k, v, ks, vs, torch.zeros(1 << 21, dtype=torch.int32, device=dev), 1 << 28)
+    i32 = dict(dtype=torch.int32, device=dev)
+    T = 1 << 30
+    many = torch.empty(T, **i32)
+    out = paged.StepPlan(cu=torch.empty(2, **i32), row=many, pos=many, slot=torch.empty(T, dtype=torch.int64, device=dev),
+                         unit=torch.empty(1026, 4, **i32), kv_len=torch.empty(1, **i32),
+                         counters=torch.empty(2, dtype=torch.int64, device=dev), info=torch.empty(4, **i32))
+    with pytest.raises(RuntimeError, match="fewer than 2\\^30 tokens"):
+        paged.plan_step(torch.ones(1, **i32), torch.zeros(1, **i32), torch.zeros(1, 1, **i32), torch.zeros(1, **i32),
+                        torch.tensor([0, 1], device=dev), page=1 << 20, max_tokens=T, out=out)
+
+
 # --------------------------------------------------------------------------- gather
 @pytest.mark.parametrize("code,page,hkv,dim,n", [("e4m3", 16, 1, 64, 1), ("int8", 64, 3, 128, 200), ("e4m3", 128, 8, 64, 1000),
                                                  ("int8", 32, 2, 64, 33), ("e4m3", 64, 2, 128, 0)])

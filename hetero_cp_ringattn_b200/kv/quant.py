@@ -9,7 +9,7 @@ round trip; the host keeps a mirror of the lengths and of the number of free pag
 
 from __future__ import annotations
 
-from typing import List, Optional, Sequence
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 
@@ -57,9 +57,9 @@ class Kv8Cache:
         """(k, v, k_scale, v_scale) of layer i."""
         return self.k[i], self.v[i], self.k_scale[i], self.v_scale[i]
 
-    def reserve(self, add: Sequence[int]) -> List[int]:
-        """Account for a step on the host: add[r] tokens for row r, negative to release it. Raises
-        `CapacityError`, changing nothing, where the device plan would not fit."""
+    def after(self, add: Sequence[int]) -> Tuple[List[int], int]:
+        """The host mirror (lengths, free pages) after a step of add[r] tokens for row r, negative to release
+        it; changes nothing. Raises `CapacityError` where the device plan would not fit."""
         if len(add) != self.rows:
             raise RingError(f"{len(add)} entries for {self.rows} rows")
         held = lambda n: -(-n // self.page)  # noqa: E731
@@ -70,7 +70,16 @@ class Kv8Cache:
         free = self.free_pages + sum(held(n) for n in self.lens) - sum(held(n) for n in new)
         if free < 0:
             raise CapacityError(f"8-bit KV cache: {-free} pages short ({self.pages} in all)")
-        self.lens, self.free_pages = new, free
+        return new, free
+
+    def commit(self, state: Tuple[List[int], int]) -> None:
+        """Take over what `after` returned. Belongs directly behind the launch of the step's plan, so that the
+        mirror never counts tokens that the device was not told about."""
+        self.lens, self.free_pages = state
+
+    def reserve(self, add: Sequence[int]) -> List[int]:
+        """Check and account for a step in one go, for callers that launch its plan next."""
+        self.commit(self.after(add))
         return [int(a) for a in add]
 
     def plan(self, add: torch.Tensor, max_tokens: int, out: Optional[paged.StepPlan] = None) -> paged.StepPlan:
@@ -82,6 +91,10 @@ class Kv8Cache:
                                max_tokens=max_tokens, out=out)
 
     def release(self, row: int) -> None:
+        if not 0 <= row < self.rows:
+            raise RingError(f"row {row}: the cache has {self.rows}")
         add = [0] * self.rows
         add[row] = -1
-        self.plan(torch.tensor(self.reserve(add), dtype=torch.int32, device=self.kv_len.device), 1)
+        state = self.after(add)
+        self.plan(torch.tensor(add, dtype=torch.int32, device=self.kv_len.device), 1)
+        self.commit(state)

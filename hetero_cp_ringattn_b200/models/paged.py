@@ -56,14 +56,19 @@ class PagedDecoder:
     @torch.no_grad()
     def prefill(self, row: int, ids: torch.Tensor, piece: int = 8192) -> torch.Tensor:
         """Append a prompt (or a session's next segment) to `row`, at most `piece` tokens at a time;
-        returns the last token's logits [vocab], float32."""
+        returns the last token's logits [vocab], float32. A prompt that does not fit is refused whole; one
+        that fails on the way leaves the row with the pieces that were appended."""
+        if not 0 <= row < self.cache.rows:
+            raise RingError(f"row {row}: the cache has {self.cache.rows}")
         if ids.numel() < 1:
             raise RingError("empty prompt")
+        if piece < 1:
+            raise RingError(f"pieces of {piece} tokens")
         add = [0] * self.cache.rows
         add[row] = int(ids.numel())
         had = self.cache.lens[row]
-        self.cache.reserve(add)
-        ids = ids.to(self.device).int()
+        self.cache.after(add)
+        ids = ids.reshape(-1).to(self.device).int()
         x = None
         for at in range(0, ids.numel(), piece):
             x = self._piece(row, ids[at:at + piece], had + at)
@@ -72,9 +77,11 @@ class PagedDecoder:
     def _piece(self, row: int, ids: torch.Tensor, had: int) -> torch.Tensor:
         w, cfg, c = self.w, self.cfg, self.cache
         T, L = ids.numel(), had + ids.numel()
-        add = torch.zeros(c.rows, dtype=torch.int32)
+        add = [0] * c.rows
         add[row] = T
-        plan = c.plan(add.to(self.device), T)
+        state = c.after(add)
+        plan = c.plan(torch.tensor(add, dtype=torch.int32, device=self.device), T)
+        c.commit(state)
         pos = torch.arange(had, L, dtype=torch.int32, device=self.device)
         x = K.embedding(ids, w.embed) if self.cuda else w.embed[ids.long()].float()
         back = [torch.empty(self.Hkv, L, self.D, dtype=torch.bfloat16, device=self.device) for _ in "kv"]
@@ -113,12 +120,17 @@ class PagedDecoder:
         add = [0] * self.cache.rows
         for r in rows:
             add[r] = 1
-        self.cache.reserve(add)
+        for name, x in (("tokens", tokens), ("u", u), ("temperature", temperature), ("top_k", top_k), ("top_p", top_p),
+                        ("min_p", min_p)):
+            single = x is not tokens and x is not u and isinstance(x, torch.Tensor) and x.dim() == 0   # a number
+            if isinstance(x, torch.Tensor) and not single and x.numel() != n:
+                raise RingError(f"{name}: {x.numel()} values for {n} rows")
+        state = self.cache.after(add)
         bucket = 1 << (n - 1).bit_length()
         st = self._steps.get(bucket)
         if st is None:
             st = self._steps[bucket] = _Step(self, bucket)
-        return st.run(n, add, tokens, u, temperature, top_k, top_p, min_p)
+        return st.run(n, add, state, tokens, u, temperature, top_k, top_p, min_p)
 
     def release(self, row: int) -> None:
         """Give the row's pages back."""
@@ -176,11 +188,13 @@ class _Step:
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.graph_launches = 0
 
-    def body(self) -> None:
+    def body(self, planned=lambda: None) -> None:
+        """The step; `planned` is called once the plan is launched."""
         d, w, cfg, c = self.d, self.d.w, self.d.cfg, self.d.cache
         eps = cfg.rms_norm_eps
         few = self.n <= GEMV_ROWS
         plan = c.plan(self.add, self.n, out=self.plan)
+        planned()
         x = self.x
         x.copy_(K.embedding(self.tokens, w.embed))
         for li, lw in enumerate(w.layers):
@@ -204,18 +218,20 @@ class _Step:
         self.logits = d._logits(x)
         sampling.sample(self.logits, self.u, *self.settings, out=self.out)
 
-    def run(self, active: int, add, tokens, u, *settings) -> torch.Tensor:
+    def run(self, active: int, add, state, tokens, u, *settings) -> torch.Tensor:
+        """The step of `add`; `state`: the cache's host mirror after it, taken over with the plan."""
+        commit = lambda: self.d.cache.commit(state)  # noqa: E731
         self.add.copy_(torch.tensor(add, dtype=torch.int32))
-        self.tokens[:active].copy_(tokens.view(-1))
+        self.tokens[:active].copy_(tokens.reshape(-1))
         for buf, value in zip(self.settings, settings):
             if isinstance(value, torch.Tensor):
-                buf[:active].copy_(value)
+                buf[:active].copy_(value.reshape(-1))
             else:
                 buf.fill_(value)
         if u is not None:
-            self.u[:active].copy_(u)
+            self.u[:active].copy_(u.reshape(-1))
         if not self.d.use_graphs:
-            self.body()
+            self.body(commit)
         else:
             if self.graph is None:
                 # nothing runs during the capture: the first replay is the first step
@@ -225,6 +241,7 @@ class _Step:
                         self.body()
                 self.graph, self.graph_launches = graph, cap.launches
             self.graph.replay()
+            commit()
             launches.count(self.graph_launches)
         self.d.last_logits = self.logits[:active]
         return self.out[:active]

@@ -314,6 +314,71 @@ def test_decoder_matches_the_quantised_oracle(code, page, bias):
         dec.prefill(1, torch.zeros(129, dtype=torch.int64))
 
 
+def _small_decoder(**kw):
+    hf = _model()
+    kw = {**dict(rows=3, max_context=64, page=16, device=torch.device("cpu")), **kw}
+    return PagedDecoder(hf.cfg, PreparedWeights.from_weights(hf, dtype=torch.float32), **kw)
+
+
+def test_refused_steps_and_prompts_change_nothing(monkeypatch):
+    """Whatever a call raises for, the host's lengths stay the device's, and the next step is as if the call
+    had not been made."""
+    dec, ref_dec = _small_decoder(), _small_decoder()
+    for d in (dec, ref_dec):
+        d.prefill(0, torch.arange(9))
+        d.prefill(2, torch.arange(5))
+    one = lambda n, v=1.0: torch.full((n,), v)  # noqa: E731
+    for kw in (dict(tokens=torch.arange(3)), dict(tokens=torch.arange(1)), dict(u=one(3)), dict(u=one(1)), dict(temperature=one(3)),
+               dict(top_k=one(1).int()), dict(top_p=one(4)), dict(min_p=one(1))):
+        with pytest.raises(RingError):
+            dec.step([0, 2], **{**dict(tokens=torch.arange(2), u=one(2, 0.5), temperature=1.0), **kw})
+    for row, ids, piece in ((-1, torch.arange(3), 16), (3, torch.arange(3), 16), (1, torch.arange(3), 0), (1, torch.arange(65), 16),
+                            (1, torch.arange(0), 16)):
+        with pytest.raises(RingError):
+            dec.prefill(row, ids, piece)
+    for row in (-1, 3):
+        with pytest.raises(RingError):
+            dec.release(row)
+    # a failure on the way to the plan
+    with monkeypatch.context() as m:
+        m.setattr(paged, "plan_step", lambda *a, **k: (_ for _ in ()).throw(MemoryError()))
+        for call in (lambda: dec.step([0, 2], torch.arange(2)), lambda: dec.prefill(1, torch.arange(20)), lambda: dec.release(0)):
+            with pytest.raises(MemoryError):
+                call()
+            assert dec.cache.lens == dec.cache.kv_len.tolist() == [9, 0, 5]
+    # and behind it: the tokens are in the cache on both sides
+    with monkeypatch.context() as m:
+        m.setattr(sampling, "sample", lambda *a, **k: (_ for _ in ()).throw(MemoryError()))
+        for d in (dec, ref_dec):
+            with pytest.raises(MemoryError):
+                d.step([0], torch.arange(1))
+            assert d.cache.lens == d.cache.kv_len.tolist() == [10, 0, 5]
+    free = dec.cache.pages - sum(-(-n // 16) for n in dec.cache.lens)
+    assert dec.cache.free_pages == free == int(dec.cache.counters[1] - dec.cache.counters[0])
+    assert torch.equal(dec.step([0, 2], torch.arange(2)), ref_dec.step([0, 2], torch.arange(2)))
+    assert torch.equal(dec.last_logits, ref_dec.last_logits)
+    number = torch.tensor(0.7)                     # a setting as a tensor of one number is for every row
+    assert torch.equal(dec.step([0, 2], torch.arange(2), one(2, 0.5), number), ref_dec.step([0, 2], torch.arange(2), one(2, 0.5), 0.7))
+
+
+def test_prompt_that_fails_between_pieces_keeps_the_mirror(monkeypatch):
+    dec = _small_decoder()
+    piece, calls = dec._piece, []
+
+    def twice(*a):
+        calls.append(a)
+        if len(calls) > 1:
+            raise MemoryError()
+        return piece(*a)
+
+    monkeypatch.setattr(dec, "_piece", twice)
+    with pytest.raises(MemoryError):
+        dec.prefill(1, torch.arange(40), piece=16)
+    assert dec.cache.lens == dec.cache.kv_len.tolist() == [0, 16, 0]
+    dec.release(1)
+    assert dec.cache.free_pages == dec.cache.pages == int(dec.cache.counters[1] - dec.cache.counters[0])
+
+
 def test_decoder_generate_is_reproducible_and_releases_its_pages():
     hf = _model()
     dec = PagedDecoder(hf.cfg, PreparedWeights.from_weights(hf, dtype=torch.float32), rows=2, max_context=64, device=torch.device("cpu"))

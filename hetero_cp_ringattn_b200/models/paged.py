@@ -125,6 +125,8 @@ class PagedDecoder:
             single = x is not tokens and x is not u and isinstance(x, torch.Tensor) and x.dim() == 0   # a number
             if isinstance(x, torch.Tensor) and not single and x.numel() != n:
                 raise RingError(f"{name}: {x.numel()} values for {n} rows")
+        if u is None and (bool((temperature > 0).any()) if isinstance(temperature, torch.Tensor) else temperature > 0):
+            raise RingError("a positive temperature needs u")
         state = self.cache.after(add)
         bucket = 1 << (n - 1).bit_length()
         st = self._steps.get(bucket)

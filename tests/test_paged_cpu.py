@@ -361,6 +361,20 @@ def test_refused_steps_and_prompts_change_nothing(monkeypatch):
     assert torch.equal(dec.step([0, 2], torch.arange(2), one(2, 0.5), number), ref_dec.step([0, 2], torch.arange(2), one(2, 0.5), 0.7))
 
 
+def test_step_with_a_temperature_needs_uniform_numbers():
+    """Without u no earlier step's numbers are drawn with; greedy steps need none."""
+    dec = _small_decoder()
+    for r in (0, 1):
+        dec.prefill(r, torch.arange(4))
+    dec.step([0, 1], torch.arange(2), torch.tensor([0.9, 0.9]), temperature=1.0)
+    for t in (1.0, torch.tensor([0.0, 0.5]), torch.tensor(2.0)):
+        with pytest.raises(RingError, match="needs u"):
+            dec.step([0, 1], torch.arange(2), temperature=t)
+    assert dec.cache.lens == [5, 5, 0]
+    for t in (0.0, -1.0, float("nan"), torch.zeros(2)):
+        assert torch.equal(dec.step([0, 1], torch.arange(2), temperature=t), dec.last_logits.argmax(-1))
+
+
 def test_prompt_that_fails_between_pieces_keeps_the_mirror(monkeypatch):
     dec = _small_decoder()
     piece, calls = dec._piece, []

@@ -13,7 +13,9 @@ Several ranks keep the bf16 arena (`models/llama.py`).
 
 from __future__ import annotations
 
+import gc
 import math
+import weakref
 from typing import Dict, List, Optional, Sequence
 
 import torch
@@ -173,7 +175,8 @@ class _Step:
     """Static buffers of a step of up to `n` active rows, and the captured step."""
 
     def __init__(self, dec: PagedDecoder, n: int):
-        self.d, self.n = dec, n
+        # (no cycle: a decoder that is given up frees its cache and graphs at once)
+        self.d, self.n = weakref.proxy(dec), n
         dev, c = dec.device, dec.cache
         self.add = torch.zeros(c.rows, dtype=torch.int32, device=dev)
         self.tokens = torch.zeros(n, dtype=torch.int32, device=dev)
@@ -238,9 +241,17 @@ class _Step:
             if self.graph is None:
                 # nothing runs during the capture: the first replay is the first step
                 graph = torch.cuda.CUDAGraph()
-                with launches.capture() as cap:
-                    with torch.cuda.graph(graph):
-                        self.body()
+                # a garbage collection inside the capture may destroy another graph, which CUDA answers by
+                # invalidating the capture
+                collects = gc.isenabled()
+                gc.disable()
+                try:
+                    with launches.capture() as cap:
+                        with torch.cuda.graph(graph):
+                            self.body()
+                finally:
+                    if collects:
+                        gc.enable()
                 self.graph, self.graph_launches = graph, cap.launches
             self.graph.replay()
             commit()

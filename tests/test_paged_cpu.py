@@ -1,9 +1,11 @@
 """The paged 8-bit KV cache, its step plan and the batched sampler on the CPU: the oracles that the
 kernels are tested against, and the single-rank decoder built on them."""
 
+import gc
 import json
 import math
 import random
+import weakref
 
 import pytest
 import torch
@@ -373,6 +375,19 @@ def test_step_with_a_temperature_needs_uniform_numbers():
     assert dec.cache.lens == [5, 5, 0]
     for t in (0.0, -1.0, float("nan"), torch.zeros(2)):
         assert torch.equal(dec.step([0, 1], torch.arange(2), temperature=t), dec.last_logits.argmax(-1))
+
+
+def test_decoder_is_freed_without_a_garbage_collection():
+    dec = _small_decoder()
+    dec.generate([torch.arange(5)] * 2, 3)
+    gone = weakref.ref(dec)
+    gc.collect()
+    gc.disable()
+    try:
+        del dec
+        assert gone() is None
+    finally:
+        gc.enable()
 
 
 def test_prompt_that_fails_between_pieces_keeps_the_mirror(monkeypatch):

@@ -754,6 +754,42 @@ def test_decoder_on_the_gpu_matches_the_quantised_oracle(dev, code, page, rows):
     assert dec.cache.kv_len.tolist() == want == dec.cache.lens
 
 
+def test_decoder_capture_survives_a_garbage_collection(dev, monkeypatch):
+    """Another decoder with a captured graph becomes unreachable, in a cycle, while a step is captured, and
+    the collector is due at every allocation."""
+    import gc
+    from hetero_cp_ringattn_b200.models.paged import PagedDecoder
+    from hetero_cp_ringattn_b200.models.weights import PreparedWeights
+    cfg = preset("tiny-gpu")
+    w = PreparedWeights.random(cfg, seed=0, device=dev)
+    prompt = torch.arange(9)
+    old = [PagedDecoder(cfg, w, rows=1, max_context=64)]
+    want = old[0].generate([prompt], 6)[0]
+    new = PagedDecoder(cfg, w, rows=1, max_context=64)
+    new.prefill(0, prompt)
+    first = want[:1]
+    append = paged.rope_append_kv8
+
+    def drop(*a, **k):
+        if old:
+            cycle = [old.pop()]
+            cycle.append(cycle)
+            del cycle
+        [[i] for i in range(100)]
+        return append(*a, **k)
+
+    monkeypatch.setattr(paged, "rope_append_kv8", drop)
+    was = gc.get_threshold()
+    gc.set_threshold(1, 1, 1)
+    try:
+        got = [first]
+        for _ in range(5):
+            got.append(new.step([0], got[-1]).clone())
+    finally:
+        gc.set_threshold(*was)
+    assert not old and torch.equal(torch.cat(got), want)
+
+
 def test_decoder_graph_equals_eager_and_is_reproducible(dev):
     from hetero_cp_ringattn_b200.models.paged import PagedDecoder
     from hetero_cp_ringattn_b200.models.weights import PreparedWeights

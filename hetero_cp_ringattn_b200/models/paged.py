@@ -52,7 +52,7 @@ class PagedDecoder:
         self.status = torch.zeros(8, dtype=torch.int32, device=self.device) if self.cuda else None
         self.use_graphs = use_graphs and self.cuda
         self._steps: Dict[int, "_Step"] = {}
-        self.last_logits: Optional[torch.Tensor] = None
+        self._logits_now: Optional[torch.Tensor] = None   # the last step's, in its buffer
 
     # ------------------------------------------------------------------ prompts
     @torch.no_grad()
@@ -114,7 +114,7 @@ class PagedDecoder:
              temperature=0.0, top_k=0, top_p=1.0, min_p=0.0) -> torch.Tensor:
         """One decode step: rows[i] (ascending) takes tokens[i] and gets its next token, int64
         [len(rows)] on the device. Settings are numbers or one value per row; `u` the uniform
-        numbers (needed when any temperature is positive). `last_logits` holds the step's logits."""
+        numbers (needed when any temperature is positive). `last_logits` are the step's logits."""
         rows = [int(r) for r in rows]
         n = len(rows)
         if n == 0 or any(b <= a for a, b in zip(rows, rows[1:])) or rows[0] < 0 or rows[-1] >= self.cache.rows:
@@ -135,6 +135,11 @@ class PagedDecoder:
         if st is None:
             st = self._steps[bucket] = _Step(self, bucket)
         return st.run(n, add, state, tokens, u, temperature, top_k, top_p, min_p)
+
+    @property
+    def last_logits(self) -> Optional[torch.Tensor]:
+        """A copy of the last step's logits [rows, vocab], which the next step may overwrite."""
+        return None if self._logits_now is None else self._logits_now.clone()
 
     def release(self, row: int) -> None:
         """Give the row's pages back."""
@@ -163,7 +168,7 @@ class PagedDecoder:
             cur = sampling.sample(torch.stack(logits), draw(), **settings)
             outs = [cur]
             for _ in range(max_new_tokens - 1):
-                cur = self.step(rows, cur, draw(), **settings).clone()
+                cur = self.step(rows, cur, draw(), **settings)
                 outs.append(cur)
         finally:
             for r in started:
@@ -256,5 +261,5 @@ class _Step:
             self.graph.replay()
             commit()
             launches.count(self.graph_launches)
-        self.d.last_logits = self.logits[:active]
-        return self.out[:active]
+        self.d._logits_now = self.logits[:active]
+        return self.out[:active].clone()     # (the next step of this size writes `out` again)

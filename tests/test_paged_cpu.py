@@ -390,6 +390,24 @@ def test_decoder_is_freed_without_a_garbage_collection():
         gc.enable()
 
 
+def check_results_stay(dec):
+    """Tokens and logits of a step do not change with later steps of the same size."""
+    vocab = dec.cfg.vocab_size
+    for r in (0, 1):
+        dec.prefill(r, torch.arange(4 + r))
+    kept = []
+    for i in range(4):
+        out = dec.step([0, 1], torch.tensor([11 * i + 1, 7 * i + 300]) % vocab)
+        kept.append((out, out.tolist(), dec.last_logits, dec.last_logits.tolist()))
+    assert len({tuple(k[1]) for k in kept}) > 1
+    for out, values, logits, logit_values in kept:
+        assert out.tolist() == values and logits.tolist() == logit_values
+
+
+def test_results_of_a_step_stay():
+    check_results_stay(_small_decoder())
+
+
 def test_prompt_that_fails_between_pieces_keeps_the_mirror(monkeypatch):
     dec = _small_decoder()
     piece, calls = dec._piece, []

@@ -790,6 +790,15 @@ def test_decoder_capture_survives_a_garbage_collection(dev, monkeypatch):
     assert not old and torch.equal(torch.cat(got), want)
 
 
+@pytest.mark.parametrize("graphs", [True, False])
+def test_decoder_results_of_a_step_stay(dev, graphs):
+    from hetero_cp_ringattn_b200.models.paged import PagedDecoder
+    from hetero_cp_ringattn_b200.models.weights import PreparedWeights
+    from test_paged_cpu import check_results_stay
+    cfg = preset("tiny-gpu")
+    check_results_stay(PagedDecoder(cfg, PreparedWeights.random(cfg, seed=0, device=dev), rows=2, max_context=64, use_graphs=graphs))
+
+
 def test_decoder_graph_equals_eager_and_is_reproducible(dev):
     from hetero_cp_ringattn_b200.models.paged import PagedDecoder
     from hetero_cp_ringattn_b200.models.weights import PreparedWeights

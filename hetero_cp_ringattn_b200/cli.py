@@ -208,7 +208,6 @@ def _infer_paged(args, dev) -> int:
                        device=dev)
     out = dec.generate([ids], max(1, args.max_tokens), temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
                        min_p=args.min_p, seed=args.seed)[0].tolist()
-    dec.check_device()
     print(json.dumps({"prompt_tokens": ids.numel(), "tokens": out, "text": tok.decode(out), "kv_cache": args.kv_cache,
                       "kv_bytes": dec.cache.bytes}))
     return 0

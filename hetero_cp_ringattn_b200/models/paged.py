@@ -21,7 +21,7 @@ from typing import Dict, List, Optional, Sequence
 import torch
 
 from ..config import ModelConfig
-from ..errors import RingError
+from ..errors import KernelError, RingError
 from ..kv.quant import Kv8Cache
 from ..ops import kernels as K
 from ..ops import paged
@@ -49,7 +49,9 @@ class PagedDecoder:
                                     scaling=cfg.rope_scaling)
         self.cos, self.sin = cos.contiguous(), sin.contiguous()
         self.act = torch.bfloat16 if self.cuda else torch.float32
+        # the kernels' error word, and its copy on the host, brought there behind every step and prompt
         self.status = torch.zeros(8, dtype=torch.int32, device=self.device) if self.cuda else None
+        self._seen = torch.zeros(8, dtype=torch.int32, pin_memory=True) if self.cuda else None
         self.use_graphs = use_graphs and self.cuda
         self._steps: Dict[int, "_Step"] = {}
         self._logits_now: Optional[torch.Tensor] = None   # the last step's, in its buffer
@@ -60,6 +62,7 @@ class PagedDecoder:
         """Append a prompt (or a session's next segment) to `row`, at most `piece` tokens at a time;
         returns the last token's logits [vocab], float32. A prompt that does not fit is refused whole; one
         that fails on the way leaves the row with the pieces that were appended."""
+        self._raise_seen()
         if not 0 <= row < self.cache.rows:
             raise RingError(f"row {row}: the cache has {self.cache.rows}")
         if ids.numel() < 1:
@@ -74,6 +77,7 @@ class PagedDecoder:
         x = None
         for at in range(0, ids.numel(), piece):
             x = self._piece(row, ids[at:at + piece], had + at)
+        self._look()
         return self._logits(x[-1:])[0].float()
 
     def _piece(self, row: int, ids: torch.Tensor, had: int) -> torch.Tensor:
@@ -85,7 +89,7 @@ class PagedDecoder:
         plan = c.plan(torch.tensor(add, dtype=torch.int32, device=self.device), T)
         c.commit(state)
         pos = torch.arange(had, L, dtype=torch.int32, device=self.device)
-        x = K.embedding(ids, w.embed) if self.cuda else w.embed[ids.long()].float()
+        x = K.embedding(ids, w.embed, status=self.status) if self.cuda else w.embed[ids.long()].float()
         back = [torch.empty(self.Hkv, L, self.D, dtype=torch.bfloat16, device=self.device) for _ in "kv"]
         for li, lw in enumerate(w.layers):
             xn = K.rmsnorm(x, lw.in_norm, cfg.rms_norm_eps)
@@ -115,6 +119,7 @@ class PagedDecoder:
         """One decode step: rows[i] (ascending) takes tokens[i] and gets its next token, int64
         [len(rows)] on the device. Settings are numbers or one value per row; `u` the uniform
         numbers (needed when any temperature is positive). `last_logits` are the step's logits."""
+        self._raise_seen()
         rows = [int(r) for r in rows]
         n = len(rows)
         if n == 0 or any(b <= a for a, b in zip(rows, rows[1:])) or rows[0] < 0 or rows[-1] >= self.cache.rows:
@@ -134,7 +139,9 @@ class PagedDecoder:
         st = self._steps.get(bucket)
         if st is None:
             st = self._steps[bucket] = _Step(self, bucket)
-        return st.run(n, add, state, tokens, u, temperature, top_k, top_p, min_p)
+        out = st.run(n, add, state, tokens, u, temperature, top_k, top_p, min_p)
+        self._look()
+        return out
 
     @property
     def last_logits(self) -> Optional[torch.Tensor]:
@@ -146,9 +153,23 @@ class PagedDecoder:
         self.cache.release(row)
 
     def check_device(self) -> None:
-        """Raise if a kernel reported an error (a page id or position out of range)."""
+        """Wait for the device and raise if a kernel reported an error since the last one raised for (a token,
+        page id or position out of range). `generate` ends with it; `prefill` and `step` raise, without
+        waiting, for what earlier ones are known to have reported."""
         if self.status is not None and int(self.status[0]):
-            raise RingError(f"device status {self.status.tolist()}")
+            word = self.status.tolist()
+            self.status.zero_()          # each report is raised once, and says nothing about later calls
+            if self._seen is not None:
+                self._seen.zero_()       # (its copies are done: the read above waited for them)
+            raise KernelError(f"device status {word}")
+
+    def _look(self) -> None:
+        if self._seen is not None:
+            self._seen.copy_(self.status, non_blocking=True)
+
+    def _raise_seen(self) -> None:
+        if self._seen is not None and int(self._seen[0]):
+            self.check_device()
 
     @torch.no_grad()
     def generate(self, prompts: Sequence[torch.Tensor], max_new_tokens: int, *, temperature=0.0, top_k=0, top_p=1.0,
@@ -170,6 +191,7 @@ class PagedDecoder:
             for _ in range(max_new_tokens - 1):
                 cur = self.step(rows, cur, draw(), **settings)
                 outs.append(cur)
+            self.check_device()
         finally:
             for r in started:
                 self.release(r)
@@ -206,7 +228,7 @@ class _Step:
         plan = c.plan(self.add, self.n, out=self.plan)
         planned()
         x = self.x
-        x.copy_(K.embedding(self.tokens, w.embed))
+        x.copy_(K.embedding(self.tokens, w.embed, status=d.status))
         for li, lw in enumerate(w.layers):
             if few:
                 qkv = K.gemv(x, lw.wqkv, "f32", bias=lw.bqkv, y_f32=self.qkv, norm_w=lw.in_norm, eps=eps)
@@ -231,7 +253,8 @@ class _Step:
     def run(self, active: int, add, state, tokens, u, *settings) -> torch.Tensor:
         """The step of `add`; `state`: the cache's host mirror after it, taken over with the plan."""
         commit = lambda: self.d.cache.commit(state)  # noqa: E731
-        self.add.copy_(torch.tensor(add, dtype=torch.int32))
+        # (from pinned memory, so the host does not wait here for the step before)
+        self.add.copy_(torch.tensor(add, dtype=torch.int32, pin_memory=self.d.cuda), non_blocking=True)
         self.tokens[:active].copy_(tokens.reshape(-1))
         for buf, value in zip(self.settings, settings):
             if isinstance(value, torch.Tensor):

@@ -11,7 +11,7 @@ import pytest
 import torch
 
 from hetero_cp_ringattn_b200.config import preset
-from hetero_cp_ringattn_b200.errors import CapacityError, RingError
+from hetero_cp_ringattn_b200.errors import CapacityError, KernelError, RingError
 from hetero_cp_ringattn_b200.kv.quant import CODES, Kv8Cache
 from hetero_cp_ringattn_b200.models.paged import PagedDecoder
 from hetero_cp_ringattn_b200.models.weights import ModelWeights, PreparedWeights
@@ -388,6 +388,17 @@ def test_decoder_is_freed_without_a_garbage_collection():
         assert gone() is None
     finally:
         gc.enable()
+
+
+def test_generate_raises_for_a_report_and_clears_it():
+    """The status word as a kernel would leave it (the CPU forms have none of their own)."""
+    dec = _small_decoder()
+    want = dec.generate([torch.arange(5)], 3)[0]
+    dec.status = torch.tensor([18, 402, 7, 0, 0, 0, 0, 0], dtype=torch.int32)
+    with pytest.raises(KernelError, match="402"):
+        dec.generate([torch.arange(5)], 3)
+    assert not dec.status.any() and dec.cache.lens == [0, 0, 0]
+    assert torch.equal(dec.generate([torch.arange(5)], 3)[0], want)
 
 
 def check_results_stay(dec):

@@ -754,6 +754,34 @@ def test_decoder_on_the_gpu_matches_the_quantised_oracle(dev, code, page, rows):
     assert dec.cache.kv_len.tolist() == want == dec.cache.lens
 
 
+@pytest.mark.parametrize("graphs", [True, False])
+def test_decoder_raises_for_what_kernels_reported(dev, graphs):
+    """A token id past the vocabulary, given to a step, a prompt and generate: raised by the next call once the
+    device has run, or by check_device and generate, once each, and the decoder goes on."""
+    from hetero_cp_ringattn_b200.errors import KernelError
+    from hetero_cp_ringattn_b200.models.paged import PagedDecoder
+    from hetero_cp_ringattn_b200.models.weights import PreparedWeights
+    cfg = preset("tiny-gpu")
+    dec = PagedDecoder(cfg, PreparedWeights.random(cfg, seed=0, device=dev), rows=2, max_context=128, use_graphs=graphs)
+    prompt, bad = torch.arange(9), torch.tensor([cfg.vocab_size])
+    want = dec.generate([prompt], 4)[0]
+    dec.prefill(0, prompt)
+    for call in (lambda: dec.step([0], bad), lambda: dec.prefill(1, bad)):
+        for after in (lambda: dec.step([0], want[:1]), lambda: dec.prefill(1, prompt), dec.check_device):
+            call()
+            torch.cuda.synchronize()
+            lens = list(dec.cache.lens)
+            with pytest.raises(KernelError, match="301"):
+                after()
+            assert dec.cache.lens == lens
+            dec.check_device()
+    for r in (0, 1):
+        dec.release(r)
+    with pytest.raises(KernelError, match="301"):
+        dec.generate([bad], 2)
+    assert torch.equal(dec.generate([prompt], 4)[0], want)
+
+
 def test_decoder_capture_survives_a_garbage_collection(dev, monkeypatch):
     """Another decoder with a captured graph becomes unreachable, in a cycle, while a step is captured, and
     the collector is due at every allocation."""

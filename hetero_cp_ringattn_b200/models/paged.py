@@ -174,11 +174,12 @@ class PagedDecoder:
     @torch.no_grad()
     def generate(self, prompts: Sequence[torch.Tensor], max_new_tokens: int, *, temperature=0.0, top_k=0, top_p=1.0,
                  min_p=0.0, seed: int = 0, piece: int = 8192) -> List[torch.Tensor]:
-        """Generate for up to `rows` prompts at once; the ids per prompt, on the device."""
-        if len(prompts) > self.cache.rows:
-            raise RingError(f"{len(prompts)} prompts for {self.cache.rows} rows")
+        """Generate for several prompts at once, each in a row that holds nothing yet and is released at the
+        end; the ids per prompt, on the device."""
+        rows = [r for r, n in enumerate(self.cache.lens) if n == 0][:len(prompts)]
+        if len(prompts) > len(rows):
+            raise RingError(f"{len(prompts)} prompts for {len(rows)} free rows")
         gen = torch.Generator(device=self.device).manual_seed(seed)
-        rows = list(range(len(prompts)))
         settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
         logits, started = [], []
         try:

@@ -401,6 +401,22 @@ def test_generate_raises_for_a_report_and_clears_it():
     assert torch.equal(dec.generate([torch.arange(5)], 3)[0], want)
 
 
+def test_generate_leaves_rows_in_use_alone():
+    """A session in row 0: prompts take other rows, and are refused where those do not suffice."""
+    dec, alone = _small_decoder(), _small_decoder()
+    for d in (dec, alone):
+        d.prefill(0, torch.arange(20))
+    prompts = [torch.arange(5), torch.arange(30, 41)]
+    got = dec.generate(prompts, 4, temperature=0.9, seed=1)
+    want = _small_decoder().generate(prompts, 4, temperature=0.9, seed=1)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert dec.cache.lens == [20, 0, 0]
+    with pytest.raises(RingError, match="2 free rows"):
+        dec.generate(prompts + prompts, 4)
+    assert torch.equal(dec.step([0], torch.tensor([3])), alone.step([0], torch.tensor([3])))
+    assert torch.equal(dec.last_logits, alone.last_logits)
+
+
 def check_results_stay(dec):
     """Tokens and logits of a step do not change with later steps of the same size."""
     vocab = dec.cfg.vocab_size

@@ -137,6 +137,9 @@ def cmd_infer(args) -> int:
         return _debug_exports(args, dev, torch.tensor(tok0.encode(text), dtype=torch.int64))
     if args.kv_cache != "bf16":
         return _infer_paged(args, dev)
+    for flag, given in (("--top-k", args.top_k > 0), ("--min-p", args.min_p > 0), ("--kv-page", args.kv_page is not None)):
+        if given:
+            raise SystemExit(f"{flag} needs --kv-cache e4m3 or int8")
     import torch.distributed as dist
     from .models.sampling import sample_token
     from .parallel.capacity import chunk_sizes
@@ -194,18 +197,22 @@ def cmd_infer(args) -> int:
 def _infer_paged(args, dev) -> int:
     """infer --kv-cache e4m3|int8: one rank, the paged 8-bit KV cache, sampling on the device."""
     from .models.paged import PagedDecoder
+    from .parallel.capacity import chunk_sizes
     from .serve.tokenizer import load_tokenizer
     if int(os.environ.get("WORLD_SIZE", "1")) != 1:
         raise SystemExit("--kv-cache e4m3|int8 runs on one rank")
     if args.export_logits:
         raise SystemExit("--export-logits needs --kv-cache bf16")
+    _init_ranks(dev, args.num_domains)
     cfg, w = _load_model(args, dev)
     tok = load_tokenizer(args.model_dir, cfg.vocab_size)
     text = open(args.prompt_file).read() if args.prompt_file else (args.prompt or "hello")
     ids = torch.tensor(tok.encode(text), dtype=torch.int64)
+    chunk_sizes(ids.numel(), 1, ratio=[int(x) for x in args.ratio.split(":")] if args.ratio else None,
+                explicit=[int(x) for x in args.chunk_sizes.split(",")] if args.chunk_sizes else None)   # (checks them)
+    page = args.kv_page or 64
     dec = PagedDecoder(cfg, w, rows=1, max_context=max(args.max_context, ids.numel() + args.max_tokens),
-                       kv_cache=args.kv_cache, page=args.kv_page, pages=-(-(ids.numel() + args.max_tokens) // args.kv_page),
-                       device=dev)
+                       kv_cache=args.kv_cache, page=page, pages=-(-(ids.numel() + args.max_tokens) // page), device=dev)
     out = dec.generate([ids], max(1, args.max_tokens), temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
                        min_p=args.min_p, seed=args.seed)[0].tolist()
     print(json.dumps({"prompt_tokens": ids.numel(), "tokens": out, "text": tok.decode(out), "kv_cache": args.kv_cache,
@@ -484,8 +491,8 @@ def build_parser() -> argparse.ArgumentParser:
     i.add_argument("--top-p", type=float, default=1.0)
     i.add_argument("--kv-cache", default="bf16", choices=["bf16", "e4m3", "int8"],
                    help="KV cache type; the 8-bit ones run on one rank")
-    i.add_argument("--kv-page", type=int, default=64, choices=[16, 32, 64, 128],
-                   help="tokens per page and scale of an 8-bit KV cache")
+    i.add_argument("--kv-page", type=int, default=None, choices=[16, 32, 64, 128],
+                   help="tokens per page and scale of an 8-bit KV cache (default 64)")
     i.add_argument("--top-k", type=int, default=0, help="keep the k most likely tokens (8-bit KV cache; 0: all)")
     i.add_argument("--min-p", type=float, default=0.0,
                    help="keep tokens of at least this share of the most likely one's probability (8-bit KV cache)")

@@ -474,3 +474,25 @@ def test_infer_on_the_8bit_cache(capsys):
     out = json.loads(capsys.readouterr().out)
     assert len(out["tokens"]) == 4 and out["kv_cache"] == "int8" and out["kv_bytes"] > 0
     assert math.isfinite(sum(out["tokens"]))
+
+
+_INFER = ["infer", "--model-preset", "tiny-gpu", "--device", "cpu", "--prompt", "ring", "--max-tokens", "3", "--max-context", "64"]
+
+
+@pytest.mark.parametrize("extra", [["--top-k", "1", "--temperature", "5"], ["--min-p", "0.2"], ["--kv-page", "16"],
+                                   ["--kv-cache", "int8", "--num-domains", "2"], ["--kv-cache", "e4m3", "--ratio", "5:5:1"],
+                                   ["--kv-cache", "int8", "--chunk-sizes", "1,1"]])
+def test_infer_refuses_flags_it_would_not_follow(extra):
+    """The 8-bit cache's sampling and page flags without it, and layouts of several ranks with it."""
+    from hetero_cp_ringattn_b200.cli import main
+    with pytest.raises((SystemExit, RingError), match="needs --kv-cache|WORLD_SIZE|for 1 domains"):
+        main(_INFER + extra)
+
+
+def test_infer_on_the_8bit_cache_with_one_domain(capsys):
+    from hetero_cp_ringattn_b200.cli import main
+    outs = []
+    for extra in ([], ["--num-domains", "1", "--ratio", "5", "--kv-page", "64"]):
+        assert main(_INFER + ["--kv-cache", "int8"] + extra) == 0
+        outs.append(json.loads(capsys.readouterr().out))
+    assert outs[0] == outs[1]

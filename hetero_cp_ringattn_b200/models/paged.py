@@ -88,13 +88,16 @@ class PagedDecoder:
         state = c.after(add)
         plan = c.plan(torch.tensor(add, dtype=torch.int32, device=self.device), T)
         c.commit(state)
+        # the blocks that this row's tokens touch: the plan's list has room for units of every row, and the
+        # append's launch goes by the list's length
+        unit = plan.unit[:-(-L // c.page) - had // c.page]
         pos = torch.arange(had, L, dtype=torch.int32, device=self.device)
         x = K.embedding(ids, w.embed, status=self.status) if self.cuda else w.embed[ids.long()].float()
         back = [torch.empty(self.Hkv, L, self.D, dtype=torch.bfloat16, device=self.device) for _ in "kv"]
         for li, lw in enumerate(w.layers):
             xn = K.rmsnorm(x, lw.in_norm, cfg.rms_norm_eps)
             qkv = K.gemm(xn, lw.wqkv, "bias" if lw.bqkv is not None else "store", bias=lw.bqkv)
-            q = paged.rope_append_kv8(qkv, self.cos, self.sin, plan.pos, plan.unit, c.block_table, *c.layer(li),
+            q = paged.rope_append_kv8(qkv, self.cos, self.sin, plan.pos, unit, c.block_table, *c.layer(li),
                                       heads=self.H, q_out=torch.empty(T, self.H, self.D, dtype=self.act, device=self.device),
                                       status=self.status)
             k, v = paged.gather_kv8(*c.layer(li), c.block_table[row], L, out=tuple(back))

@@ -94,7 +94,9 @@ def rope_append_kv8(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos
     write q out and code k and v into the rows' blocks.
 
     `qkv` [tokens, (heads + 2 kv_heads) * D] in float32, bf16 or f16; `pos`, `unit` of the step's plan
-    (`plan_step`, or the same lists made elsewhere). Block scales: a new block's follows from its new
+    (`plan_step`, or the same lists made elsewhere; entries with row -1 are skipped). Whole blocks are stored
+    from 12 tokens an entry of `unit` on, so a prompt's list should not be much longer than its blocks: pass
+    the part in use. Block scales: a new block's follows from its new
     tokens, an open block's grows with them (its stored codes are rescaled). Returns q [tokens, heads, D]
     in `q_out`'s type (default: qkv's, bf16 for float32). A token whose position lies outside the rotary
     tables gets q = 0, and a unit whose row, tokens, positions or page id are out of range stores nothing;

@@ -435,6 +435,26 @@ def test_results_of_a_step_stay():
     check_results_stay(_small_decoder())
 
 
+@pytest.mark.parametrize("had,n", [(0, 1), (0, 16), (0, 17), (5, 11), (5, 12), (15, 2), (16, 40), (20, 64)])
+def test_prompt_hands_the_append_its_own_units(monkeypatch, had, n):
+    """However many rows the cache has: exactly the blocks that the piece touches, all of its tokens."""
+    dec = _small_decoder(rows=40, max_context=128)
+    if had:
+        dec.prefill(3, torch.arange(had))
+    append, seen = paged.rope_append_kv8, []
+
+    def spy(qkv, cos, sin, pos, unit, *a, **k):
+        seen.append(unit.tolist())
+        return append(qkv, cos, sin, pos, unit, *a, **k)
+
+    monkeypatch.setattr(paged, "rope_append_kv8", spy)
+    dec.prefill(3, torch.arange(n))
+    assert len(seen) == dec.cfg.num_layers
+    for units in seen:
+        assert [u[3] // 16 for u in units] == list(range(had // 16, (had + n - 1) // 16 + 1))
+        assert all(u[0] == 3 for u in units) and sum(u[2] for u in units) == n
+
+
 def test_prompt_that_fails_between_pieces_keeps_the_mirror(monkeypatch):
     dec = _small_decoder()
     piece, calls = dec._piece, []

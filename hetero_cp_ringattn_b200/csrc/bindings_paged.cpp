@@ -124,7 +124,7 @@ void plan_step(const Tensor& add, const Tensor& kv_len, const Tensor& table, con
   HCP_CHECK_OK(hcp::kv8::plan_step(a, cur_stream()));
 }
 
-Tensor rope_append_kv8(const Tensor& x, const Tensor& cos_t, const Tensor& sin_t, const Tensor& pos, const Tensor& unit,
+std::tuple<Tensor, int> rope_append_kv8(const Tensor& x, const Tensor& cos_t, const Tensor& sin_t, const Tensor& pos, const Tensor& unit,
                        const Tensor& table, const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs, int64_t heads,
                        optional<Tensor> q_out, optional<Tensor> status) {
   hcp::kv8::AppendArgs a{};
@@ -169,8 +169,9 @@ Tensor rope_append_kv8(const Tensor& x, const Tensor& cos_t, const Tensor& sin_t
   a.width = int(table.size(1));
   a.q_out = out.data_ptr();
   a.status = status_ptr(status, dev);
-  HCP_CHECK_OK(hcp::kv8::rope_append(a, cur_stream()));
-  return out;
+  int launched = 0;
+  HCP_CHECK_OK(hcp::kv8::rope_append(a, cur_stream(), &launched));
+  return {out, launched};
 }
 
 std::tuple<Tensor, Tensor> gather_kv8(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs, const Tensor& table, int64_t n,

@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 4) rope_q_kernel(AppendArgs a) {
 }
 
 template <int DT, int D, bool INT8>
-cudaError_t launch_append(const AppendArgs& a, cudaStream_t s) {
+cudaError_t launch_append(const AppendArgs& a, cudaStream_t s, int* launched) {
   const long items = (long)a.T * (D / 16) * ((a.H + kQHeads - 1) / kQHeads);
   const long q_ctas = (items + kThreads - 1) / kThreads;
   if (items + kThreads > 0x7fffffffl || (long)a.U * 2 * a.c.Hkv > 0x3fffffffl) return cudaErrorInvalidValue;
@@ -324,6 +324,7 @@ cudaError_t launch_append(const AppendArgs& a, cudaStream_t s) {
   // 2048 tokens 30.7 and 19.4.
   if ((long)a.T < 12l * a.U || a.U == 0) {
     const long warps = (long)a.U * 2 * a.c.Hkv, s_ctas = (warps + kThreads / 32 - 1) / (kThreads / 32);
+    *launched = 1;
     return launch_pdl(append_short_kernel<DT, D, INT8>, dim3(unsigned(q_ctas + s_ctas)), dim3(kThreads), 0, s, a, int(s_ctas));
   }
   const int team = block_threads(a.c.P, D), threads = team > 256 ? team : 256, per = threads / team;
@@ -333,17 +334,18 @@ cudaError_t launch_append(const AppendArgs& a, cudaStream_t s) {
   const long teams = (long)a.U * 2 * ((a.c.Hkv + heads - 1) / heads);
   cudaError_t e = launch_pdl(append_block_kernel<DT, D, INT8>, dim3(unsigned((teams + per - 1) / per)), dim3(threads), 0, s, a, heads);
   if (e != cudaSuccess) return e;
+  *launched = 2;
   return launch_pdl(rope_q_kernel<DT, D>, dim3(unsigned(q_ctas)), dim3(kThreads), 0, s, a);
 }
 
 template <int DT, int D>
-cudaError_t append_code(const AppendArgs& a, cudaStream_t s) {
-  return a.c.code == kInt8 ? launch_append<DT, D, true>(a, s) : launch_append<DT, D, false>(a, s);
+cudaError_t append_code(const AppendArgs& a, cudaStream_t s, int* launched) {
+  return a.c.code == kInt8 ? launch_append<DT, D, true>(a, s, launched) : launch_append<DT, D, false>(a, s, launched);
 }
 
 template <int DT>
-cudaError_t append_dim(const AppendArgs& a, cudaStream_t s) {
-  return a.c.D == 64 ? append_code<DT, 64>(a, s) : append_code<DT, 128>(a, s);
+cudaError_t append_dim(const AppendArgs& a, cudaStream_t s, int* launched) {
+  return a.c.D == 64 ? append_code<DT, 64>(a, s, launched) : append_code<DT, 128>(a, s, launched);
 }
 
 // 16 codes of one (row, head) a thread.
@@ -399,12 +401,15 @@ const char* check_cache(const Cache& c) {
 
 }  // namespace
 
-const char* rope_append(const AppendArgs& a, cudaStream_t s) {
+const char* rope_append(const AppendArgs& a, cudaStream_t s, int* launched) {
+  *launched = 0;
   if (const char* e = check_cache(a.c)) return e;
   if (a.T < 1) return nullptr;
   if (a.row_stride % 8 || reinterpret_cast<uintptr_t>(a.x) % 16 || reinterpret_cast<uintptr_t>(a.q_out) % 16)
     return "rope_append_kv8: rows must start on 16-byte boundaries";
-  cudaError_t e = a.dtype == kF32 ? append_dim<kF32>(a, s) : a.dtype == kBF16 ? append_dim<kBF16>(a, s) : append_dim<kF16>(a, s);
+  cudaError_t e = a.dtype == kF32    ? append_dim<kF32>(a, s, launched)
+                  : a.dtype == kBF16 ? append_dim<kBF16>(a, s, launched)
+                                     : append_dim<kF16>(a, s, launched);
   return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
 }
 

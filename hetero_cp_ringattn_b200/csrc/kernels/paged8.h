@@ -66,7 +66,8 @@ struct AppendArgs {
   int q_dtype;           // kBF16 or kF16
   int* status;
 };
-const char* rope_append(const AppendArgs& a, cudaStream_t s);
+// Sets `launched` to the number of kernels.
+const char* rope_append(const AppendArgs& a, cudaStream_t s, int* launched);
 
 struct GatherArgs {
   Cache c;

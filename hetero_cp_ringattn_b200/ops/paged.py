@@ -103,8 +103,9 @@ def rope_append_kv8(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos
     both are reported to `status`, an int32 [>= 4] error word (on the CPU they raise and nothing is written)."""
     if not qkv.is_cuda:
         return pref.rope_append_kv8(qkv, cos, sin, pos, unit, block_table, k, v, k_scale, v_scale, heads, q_out)
-    q = native().rope_append_kv8(qkv, cos, sin, pos, unit, block_table, k, v, k_scale, v_scale, heads, q_out, status)
-    launches.count(2 if qkv.shape[0] >= 4 * unit.shape[0] > 0 else 1)   # prompts: k and v, then q
+    q, launched = native().rope_append_kv8(qkv, cos, sin, pos, unit, block_table, k, v, k_scale, v_scale, heads, q_out,
+                                           status)
+    launches.count(launched)
     return q
 
 
@@ -129,7 +130,7 @@ def attention_kv8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: to
         return pref.attention_kv8(q, k, v, k_scale, v_scale, block_table, kv_len, cu, scale, out, want_lse)
     o, lse = native().attention_kv8(q, k, v, k_scale, v_scale, block_table, kv_len, cu, max_q, scale, out,
                                     want_lse, status)
-    launches.count(2)
+    launches.count(2 if q.shape[0] else 0)
     return o, (lse if want_lse else None)
 
 
@@ -143,5 +144,5 @@ def gather_kv8(k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale:
             out = tuple(torch.empty(k.shape[1], n, k.shape[3], dtype=torch.bfloat16) for _ in "kv")
         return pref.gather_kv8(k, v, k_scale, v_scale, block_table_row, n, out)
     out = native().gather_kv8(k, v, k_scale, v_scale, block_table_row, n, *(out or (None, None)))
-    launches.count()
+    launches.count(1 if n else 0)
     return out

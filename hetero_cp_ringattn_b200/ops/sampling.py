@@ -43,7 +43,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 1.0, to
     p = (top_p, 0.0) if isinstance(top_p, torch.Tensor) else (None, top_p)
     m = (min_p, 0.0) if isinstance(min_p, torch.Tensor) else (None, min_p)
     token = native().sample(logits, u, *t, *k, *p, *m, out)
-    launches.count()
+    launches.count(1 if logits.shape[0] else 0)
     return token
 
 

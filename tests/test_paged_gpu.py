@@ -715,6 +715,48 @@ def test_sample_refusals(dev):
             sampling.sample(*args)
 
 
+# --------------------------------------------------------------------------- launch counts
+def _kernels_and_count(fn):
+    """Nodes of the CUDA graph that `fn` captures, and what it counted."""
+    import ctypes
+    from hetero_cp_ringattn_b200.utils import launches
+    fn()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with launches.capture() as cap:
+        with torch.cuda.graph(graph):
+            fn()
+    n = ctypes.c_size_t()
+    assert ctypes.CDLL("libcuda.so.1").cuGraphGetNodes(ctypes.c_void_p(graph.raw_cuda_graph()), None, ctypes.byref(n)) == 0
+    return n.value, cap.launches
+
+
+@pytest.mark.parametrize("tokens,units", [(0, 1), (1, 1), (3, 1), (4, 1), (8, 1), (11, 1), (12, 1), (16, 1), (16, 0), (47, 4), (48, 4)])
+def test_append_counts_what_it_launches(dev, tokens, units):
+    k, v, ks, vs = _strided_cache(4, 1, 16, 64, "e4m3", dev)
+    cos, sin = (t.to(dev) for t in ref.rope_cos_sin(torch.arange(64), 64, 10000.0))
+    x = torch.randn(tokens, 3 * 64, device=dev)
+    pos = torch.arange(tokens, dtype=torch.int32, device=dev)
+    unit = torch.tensor([[0, 16 * i, min(16, tokens - 16 * i), 16 * i] if 16 * i < tokens else [-1, 0, 0, 0] for i in range(units)],
+                        dtype=torch.int32, device=dev).view(units, 4)
+    table = torch.arange(4, dtype=torch.int32, device=dev).view(1, 4)
+    nodes, counted = _kernels_and_count(lambda: paged.rope_append_kv8(x, cos, sin, pos, unit, table, k, v, ks, vs, heads=1))
+    assert counted == nodes == (0 if tokens == 0 else 2 if 0 < 12 * units <= tokens else 1)
+
+
+@pytest.mark.parametrize("n", [0, 1, 5])
+def test_other_operators_count_what_they_launch(dev, n):
+    k, v, ks, vs = _strided_cache(2, 1, 16, 64, "int8", dev)
+    table = torch.zeros(max(n, 1), 1, dtype=torch.int32, device=dev)
+    q = torch.randn(n, 2, 64, device=dev).bfloat16()
+    lens, cu = torch.ones(max(n, 1), dtype=torch.int32, device=dev), torch.arange(max(n, 1) + 1, dtype=torch.int32, device=dev)
+    cu *= n > 0
+    x, u = torch.randn(n, 100, device=dev), torch.rand(n, device=dev)
+    for fn in (lambda: paged.attention_kv8(q, k, v, ks, vs, table, lens, cu), lambda: paged.gather_kv8(k, v, ks, vs, table[0], n),
+               lambda: sampling.sample(x, u)):
+        nodes, counted = _kernels_and_count(fn)
+        assert nodes == counted
+
+
 # --------------------------------------------------------------------------- the decoder
 @pytest.mark.parametrize("code,page,rows", [("e4m3", 64, 3), ("int8", 16, 10)])
 def test_decoder_on_the_gpu_matches_the_quantised_oracle(dev, code, page, rows):

@@ -169,6 +169,7 @@ std::tuple<Tensor, int> rope_append_kv8(const Tensor& x, const Tensor& cos_t, co
   a.width = int(table.size(1));
   a.q_out = out.data_ptr();
   a.status = status_ptr(status, dev);
+  a.num_sms = sm_count(dev.index());
   int launched = 0;
   HCP_CHECK_OK(hcp::kv8::rope_append(a, cur_stream(), &launched));
   return {out, launched};

@@ -330,7 +330,7 @@ cudaError_t launch_append(const AppendArgs& a, cudaStream_t s, int* launched) {
   const int team = block_threads(a.c.P, D), threads = team > 256 ? team : 256, per = threads / team;
   // heads a team goes through: as many as leave four CTAs an SM
   int heads = 1;
-  while (heads < a.c.Hkv && (long)a.U * 2 * (a.c.Hkv / (2 * heads)) >= 4l * 148 * per) heads *= 2;
+  while (heads < a.c.Hkv && (long)a.U * 2 * (a.c.Hkv / (2 * heads)) >= 4l * a.num_sms * per) heads *= 2;
   const long teams = (long)a.U * 2 * ((a.c.Hkv + heads - 1) / heads);
   cudaError_t e = launch_pdl(append_block_kernel<DT, D, INT8>, dim3(unsigned((teams + per - 1) / per)), dim3(threads), 0, s, a, heads);
   if (e != cudaSuccess) return e;

@@ -65,6 +65,7 @@ struct AppendArgs {
   void* q_out;           // [T][H][D]
   int q_dtype;           // kBF16 or kF16
   int* status;
+  int num_sms;
 };
 // Sets `launched` to the number of kernels.
 const char* rope_append(const AppendArgs& a, cudaStream_t s, int* launched);

@@ -191,6 +191,47 @@ def test_append_reports_and_skips_bad_places(dev):
         assert int(st[0]) == 18 and torch.equal(k.view(torch.uint8), before)
 
 
+@pytest.mark.parametrize("dtype,code,page,heads,hkv,dim,old,news", [
+    # many blocks: teams that go through several KV heads, the next one's values fetched ahead
+    (torch.bfloat16, "e4m3", 64, 8, 8, 128, [0, 37, 63, 1], [9000, 5001, 1500, 900]),
+    (torch.bfloat16, "int8", 64, 4, 5, 128, [17, 0], [9000, 3333]),          # 5 heads: a last group of fewer
+    (torch.float32, "e4m3", 64, 3, 3, 64, [5], [20011]),
+    (torch.float16, "int8", 128, 2, 7, 64, [127, 3], [20000, 801]),
+    # several teams a CTA (pages of 16 and 32), whole blocks and open ones, one head and several
+    (torch.bfloat16, "e4m3", 16, 4, 2, 128, [0, 15], [160, 97]), (torch.float32, "int8", 16, 2, 3, 64, [9], [333]),
+    (torch.float16, "e4m3", 32, 4, 1, 128, [31, 2, 0], [64, 500, 33]), (torch.bfloat16, "int8", 32, 2, 6, 64, [1], [1000]),
+    (torch.bfloat16, "e4m3", 16, 2, 8, 64, [3, 0], [9001, 4000]), (torch.float32, "e4m3", 32, 2, 5, 128, [30], [9999]),
+    (torch.float32, "int8", 16, 2, 7, 128, [8], [7000])])
+def test_append_of_prompts_equals_the_oracle(dev, dtype, code, page, heads, hkv, dim, old, news):
+    """Prompts of whole blocks behind open ones, whose stored codes are rescaled: codes, scales and q bit
+    for bit, with nothing else in the cache changed."""
+    g = torch.Generator().manual_seed(page + hkv + dim)
+    rows, width = len(old), max(-(-(o + n) // page) for o, n in zip(old, news)) + 1
+    pages = rows * width + 3
+    table = torch.randperm(pages, generator=g)[:rows * width].view(rows, width).to(torch.int32)
+    units, pos, t = [], [], 0
+    for r, (o, n) in enumerate(zip(old, news)):
+        p = o
+        while p < o + n:
+            m = min(o + n, (p // page + 1) * page) - p
+            units.append([r, t, m, p])
+            t, p = t + m, p + m
+        pos.append(torch.arange(o, o + n))
+    T, unit, pos = t, torch.tensor(units, dtype=torch.int32), torch.cat(pos).to(torch.int32)
+    assert T >= 12 * len(units)
+    x = (torch.randn(T, (heads + 2 * hkv) * dim, generator=g) * 2.0 ** torch.randint(-4, 5, (T, 1), generator=g)).to(dtype)
+    cos, sin = ref.rope_cos_sin(torch.arange(width * page), dim, 500000.0)
+    k, v, ks, vs = _strided_cache(pages, hkv, page, dim, code, dev)
+    kc, vc, ksc, vsc = (c.cpu().clone() for c in (k, v, ks, vs))
+    want = paged.rope_append_kv8(x, cos, sin, pos, unit, table, kc, vc, ksc, vsc, heads=heads)
+    st = status_tensor(dev)
+    got = paged.rope_append_kv8(x.to(dev), cos.to(dev), sin.to(dev), pos.to(dev), unit.to(dev), table.to(dev), k, v, ks, vs,
+                                heads=heads, status=st)
+    assert same(got, want) and int(st[0]) == 0
+    for a, b in ((ks, ksc), (vs, vsc), (k, kc), (v, vc)):
+        assert same(a, b)
+
+
 @pytest.mark.parametrize("n,page", [(2, 16), (16, 16), (33, 64)])
 @pytest.mark.parametrize("shift", [-1, 1])
 def test_append_writes_nothing_past_the_rotary_tables(dev, n, page, shift):

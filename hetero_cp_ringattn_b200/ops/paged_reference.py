@@ -144,7 +144,7 @@ def cached_rows(data, scale, table_row, n: int, dtype=torch.float32) -> torch.Te
     P = data.shape[2]
     pages = table_row[: -(-n // P)].long()
     raw = data.view(torch.uint8)[pages].view(data.dtype)
-    x = raw.to(torch.float32).to(dtype) * scale[pages].to(dtype).view(len(pages), -1, 1, 1)
+    x = raw.to(torch.float32).to(dtype) * scale[pages].to(dtype).view(len(pages), data.shape[1], 1, 1)
     return x.transpose(1, 2).reshape(-1, data.shape[1], data.shape[3])[:n]
 
 

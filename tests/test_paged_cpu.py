@@ -174,6 +174,13 @@ def test_scale_is_the_smallest_power_of_two_that_holds_the_maximum():
         assert s[3] == s[4] == 2.0 ** -40 and s[5] == 2.0 ** 40
 
 
+def test_gather_of_no_rows():
+    c = Kv8Cache(1, 2, 64, rows=1, max_context=48, page=16)
+    out = tuple(torch.full((2, 3, 64), 7.0, dtype=torch.bfloat16) for _ in "kv")
+    for k, v in (paged.gather_kv8(*c.layer(0), c.block_table[0], 0), paged.gather_kv8(*c.layer(0), c.block_table[0], 0, out=out)):
+        assert k.shape == v.shape and (k == 7).all() and (v == 7).all()
+
+
 # --------------------------------------------------------------------------- sampling
 def _naive(logits, u, T, k, p, m):
     """The definition by float64 weights and an explicit loop."""

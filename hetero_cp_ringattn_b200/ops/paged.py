@@ -119,7 +119,8 @@ def attention_kv8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: to
     Request b has the query tokens cu[b] .. cu[b + 1] - 1 (None: token b) and kv_len[b] cached rows; its
     query token i of m sees rows 0 .. kv_len[b] - m + i. `max_q` is the most query tokens that a request
     has: the tiles' shape goes by it, the results do not (a request with more is right, but slower). `cu`
-    past the tokens of q is reported to `status`. Returns (o [tokens, heads, D], lse [heads, tokens] natural
+    past the tokens of q and page ids outside the pool (read as zeros) are reported to `status`; on the CPU
+    they raise. Returns (o [tokens, heads, D], lse [heads, tokens] natural
     log, or None); a token that sees no row gets o = 0, lse = -inf, so the partials of several ranks' shards
     merge like the other attention's (`reference.merge_partials`). At most 1024 requests a call. Meant for
     decode steps and short segments (drafts to verify): for a long segment read the rows back with
@@ -138,7 +139,8 @@ def gather_kv8(k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale:
                block_table_row: torch.Tensor, n: int,
                out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """The first n cached rows of one request as bf16 K and V [kv_heads, n or more, D] in position order,
-    what `kernels.attention` reads. `out`: buffers to write into."""
+    what `kernels.attention` reads. `out`: buffers to write into. Rows of a page id outside the pool are
+    zeros (on the CPU they raise)."""
     if not k.is_cuda:
         if out is None:
             out = tuple(torch.empty(k.shape[1], n, k.shape[3], dtype=torch.bfloat16) for _ in "kv")

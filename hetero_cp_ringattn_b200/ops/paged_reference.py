@@ -143,6 +143,8 @@ def cached_rows(data, scale, table_row, n: int, dtype=torch.float32) -> torch.Te
     """The values of the first n cached rows, [n, kv_heads, D]."""
     P = data.shape[2]
     pages = table_row[: -(-n // P)].long()
+    if len(pages) and not 0 <= int(pages.min()) <= int(pages.max()) < data.shape[0]:
+        raise RingError(f"a page id outside the pool of {data.shape[0]} pages")   # (the kernels report and read zeros)
     raw = data.view(torch.uint8)[pages].view(data.dtype)
     x = raw.to(torch.float32).to(dtype) * scale[pages].to(dtype).view(len(pages), data.shape[1], 1, 1)
     return x.transpose(1, 2).reshape(-1, data.shape[1], data.shape[3])[:n]

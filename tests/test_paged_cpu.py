@@ -181,6 +181,23 @@ def test_gather_of_no_rows():
         assert k.shape == v.shape and (k == 7).all() and (v == 7).all()
 
 
+@pytest.mark.parametrize("bad", [-1, 3])
+def test_readers_refuse_page_ids_outside_the_pool(bad):
+    c = Kv8Cache(1, 1, 64, rows=1, max_context=48, page=16, pages=3)
+    k, v, ks, vs = c.layer(0)
+    q, lens = torch.randn(1, 2, 64), lambda n: torch.tensor([n], dtype=torch.int32)
+    for row, n, ok in (([0, 2, bad], 33, False), ([0, bad, 1], 20, False), ([0, 2, bad], 32, True), ([bad, bad, bad], 0, True)):
+        table = torch.tensor([row], dtype=torch.int32)
+        for call in (lambda: paged.attention_kv8(q, k, v, ks, vs, table, lens(n)), lambda: paged.gather_kv8(k, v, ks, vs, table[0], n)):
+            if ok:
+                call()
+            else:
+                with pytest.raises(RingError, match="page id"):
+                    call()
+    with pytest.raises((RingError, IndexError)):
+        paged.attention_kv8(q, k, v, ks, vs, torch.tensor([[0, 1, 2]], dtype=torch.int32), lens(3), torch.tensor([0, 2]))
+
+
 # --------------------------------------------------------------------------- sampling
 def _naive(logits, u, T, k, p, m):
     """The definition by float64 weights and an explicit loop."""

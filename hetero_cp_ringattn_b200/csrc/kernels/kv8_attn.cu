@@ -176,13 +176,22 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// (a call: inlined, 8 requests of up to 4096 rows took 16.8 us instead of 16.6)
+__device__ __noinline__ void offsets_out_of_range(int* status, int to, int b) {
+  report_error(status, int(StatusCode::kOutOfBounds), 413, to, b);
+}
+
 __device__ __forceinline__ int q_tokens(const AttnArgs& a, int b, int& first) {
   if (a.cu == nullptr) {
     first = b;
     return 1;
   }
-  first = max(a.cu[b], 0);
-  return max(0, min(a.cu[b + 1], a.T) - first);
+  const int from = a.cu[b], to = a.cu[b + 1];
+  first = max(from, 0);
+  const int n = max(0, min(to, a.T) - first);
+  // tokens that q does not hold would move the causal limits of those it holds
+  if (n != to - from) offsets_out_of_range(a.status, to, b);
+  return n;
 }
 
 // Cached rows of request b, no more than its table row can hold.
@@ -271,9 +280,6 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
     for (int b = r0; b < r1; ++b) {
       int first;
       s_first[a.B + b] = q_tokens(a, b, first);
-      // tokens that q does not hold would move the causal limit of those it holds
-      if (blockIdx.x == 0 && a.cu != nullptr && (a.cu[b] < 0 || a.cu[b + 1] < a.cu[b] || a.cu[b + 1] > a.T))
-        report_error(a.status, int(StatusCode::kOutOfBounds), 413, a.cu[b + 1], b);
       s_first[b] = first;
       s_rows[b] = rows_of(a, b);
       own += tiles_of(b);

@@ -10,7 +10,9 @@
 // roles swapped: S^T = K Q^T and O^T = V^T P^T, the cached tokens (or head dims) on the 16-row side
 // and up to 8 query rows a column tile, half the MMAs and accumulators that 16 padded query rows
 // would take. 8-bit codes convert to f16 exactly, so K and V enter the products unrounded:
-//   K   scales multiply the 32-bit scores; q is brought to f16 range by a power of two per row.
+//   K   scales multiply the 32-bit scores; q is brought to f16 range by a power of two per item (the
+//       query rows of one request that share a KV head): bf16's 8 bits stay exact down to 2^-31 of the
+//       item's largest element, f16's 11 to 2^-28, and below the error is 2^-39 of it.
 //   V   the scale moves into the exponent: p = 2^(s + log2 vs - m + 15) with m the running maximum
 //       of s + log2 vs, O += p Vc, l += p / vs. So one page's scale costs one addition a score, and
 //       no accumulator is rescaled for it. The 2^15 puts p's f16 rounding (2^-11 relative) down to
@@ -479,7 +481,7 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
       }
     };
     // |q| 2^e in [2^14, 2^15) for the item's largest finite element: bf16's 8 bits stay exact in f16
-    // down to 2^-32 of it
+    // down to 2^-31 of it
     float top_q = 0.f;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -574,6 +576,8 @@ attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CU
         const int half = halves == 2 ? (g0 + mt) & 1 : 0;
         const float ks = meta[stream][k_stage][half][0], vs = meta[stream][k_stage][half][1];
         // a block scaled by 0 holds zeros: its weight counts in l and its p V is 0 whatever p is
+        // (the approximate logarithm and quotient are off by a few units of the last place: a page's
+        // weights by about 2^-20, in the sum and in O alike, where P's rounding to f16 is 2^-12)
         dead[mt] = vs == 0.f || idle;
         const float lv = dead[mt] ? 0.f : __log2f(vs);
         iv[mt] = dead[mt] ? 1.f : __fdividef(1.f, vs);
@@ -1002,7 +1006,7 @@ bool make_map(CUtensorMap* map, const uint8_t* base, const Cache& c) {
 // Column tiles of 8 query rows an item has: the least that hold a request's rows, at most 5. 64 requests
 // of up to 32768 rows, 4 KV heads, 128 dims: 7 rows with 1, 2, 3 and 5 tiles 128, 155, 202, 280 us; 14
 // rows with 2, 3, 5 167, 210, 290; 21 rows with 3 and 5 220 and 302. 64 dims: 83, 101, 157, 200; 109,
-// 165, 208; 171 and 216.
+// 165, 208; 171 and 216. There is no shape of 4 tiles: 25 to 32 rows take that of 5.
 int column_tiles(const AttnArgs& a) {
   const long rows = (long)a.max_q * (a.H / a.c.Hkv);
   return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 5;

@@ -319,7 +319,7 @@ cudaError_t launch_append(const AppendArgs& a, cudaStream_t s, int* launched) {
   const long items = (long)a.T * (D / 16) * ((a.H + kQHeads - 1) / kQHeads);
   const long q_ctas = (items + kThreads - 1) / kThreads;
   if (items + kThreads > 0x7fffffffl || (long)a.U * 2 * a.c.Hkv > 0x3fffffffl) return cudaErrorInvalidValue;
-  // Whole blocks from 12 tokens a unit on average: 64 rows of 8 heads and 128 dims take 10.2 us in short
+  // Whole blocks from 12 tokens a unit on average (entries that pad the list count): 64 rows of 8 heads and 128 dims take 10.2 us in short
   // units and 19.5 us in blocks at 1 token a row, 16.4 and 21.5 at 8, 26.6 and 23.6 at 16; 5 rows of
   // 2048 tokens 30.7 and 19.4.
   if ((long)a.T < 12l * a.U || a.U == 0) {

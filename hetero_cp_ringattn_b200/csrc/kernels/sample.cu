@@ -22,8 +22,10 @@
 // 512 of them (a large k, a flat row, ties) take the general way: histograms of the crossing bin until
 // it is small, or the exact tie, then one pass over the kept tokens.
 //
-// Bound: instructions per token (distance, weight) for many rows, the chain of cluster barriers for
-// one. The weight's polynomial runs on packed pairs. Measured on B200, float32 logits: one row of
+// Bound: the phases of a row, one after another: its load, the cluster's maximum, the work on its
+// tokens, further cluster barriers. One row is that chain; of many rows two CTAs an SM overlap two chains,
+// which fills neither pipe (issue slots 33%, DRAM 9%, as many stalls on barriers as on fixed latencies).
+// The weight's polynomial runs on packed pairs. Measured on B200, float32 logits: one row of
 // 128256 tokens 20 us; 129 rows of 151936 (78 MB, 12 us of reading) 102 us with mixed settings, greedy
 // alone 32, temperature alone 62, top-k 40 70, top-k 1000 119, top-p 0.9 over random logits (the
 // general way) 183. One CTA a row that reads the row again in every pass instead of holding it: 289.

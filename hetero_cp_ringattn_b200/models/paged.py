@@ -49,9 +49,10 @@ class PagedDecoder:
                                     scaling=cfg.rope_scaling)
         self.cos, self.sin = cos.contiguous(), sin.contiguous()
         self.act = torch.bfloat16 if self.cuda else torch.float32
-        # the kernels' error word, and its copy on the host, brought there behind every step and prompt
-        self.status = torch.zeros(8, dtype=torch.int32, device=self.device) if self.cuda else None
-        self._seen = torch.zeros(8, dtype=torch.int32, pin_memory=True) if self.cuda else None
+        # the kernels' error words (see `_word`), and their copy on the host, brought there behind every step
+        # and prompt
+        self.status = torch.zeros(16, dtype=torch.int32, device=self.device) if self.cuda else None
+        self._seen = torch.zeros(16, dtype=torch.int32, pin_memory=True) if self.cuda else None
         self.use_graphs = use_graphs and self.cuda
         self._steps: Dict[int, "_Step"] = {}
         self._logits_now: Optional[torch.Tensor] = None   # the last step's, in its buffer
@@ -92,16 +93,16 @@ class PagedDecoder:
         # append's launch goes by the list's length
         unit = plan.unit[:-(-L // c.page) - had // c.page]
         pos = torch.arange(had, L, dtype=torch.int32, device=self.device)
-        x = K.embedding(ids, w.embed, status=self.status) if self.cuda else w.embed[ids.long()].float()
+        x = K.embedding(ids, w.embed, status=self._word(0)) if self.cuda else w.embed[ids.long()].float()
         back = [torch.empty(self.Hkv, L, self.D, dtype=torch.bfloat16, device=self.device) for _ in "kv"]
         for li, lw in enumerate(w.layers):
             xn = K.rmsnorm(x, lw.in_norm, cfg.rms_norm_eps)
             qkv = K.gemm(xn, lw.wqkv, "bias" if lw.bqkv is not None else "store", bias=lw.bqkv)
             q = paged.rope_append_kv8(qkv, self.cos, self.sin, plan.pos, unit, c.block_table, *c.layer(li),
                                       heads=self.H, q_out=torch.empty(T, self.H, self.D, dtype=self.act, device=self.device),
-                                      status=self.status)
+                                      status=self._word(0))
             k, v = paged.gather_kv8(*c.layer(li), c.block_table[row], L, out=tuple(back))
-            o, _ = K.attention(q, k, v, pos, L, scale=self.scale, want_lse=False, status=self.status)
+            o, _ = K.attention(q, k, v, pos, L, scale=self.scale, want_lse=False, status=self._word(1))
             x = K.gemm(o.reshape(T, -1), lw.wo, "residual", residual=x)
             g = K.gemm(K.rmsnorm(x, lw.post_norm, cfg.rms_norm_eps), lw.wgu, "swiglu")
             x = K.gemm(g, lw.wd, "residual", residual=x)
@@ -159,19 +160,24 @@ class PagedDecoder:
         """Wait for the device and raise if a kernel reported an error since the last one raised for (a token,
         page id or position out of range). `generate` ends with it; `prefill` and `step` raise, without
         waiting, for what earlier ones are known to have reported."""
-        if self.status is not None and int(self.status[0]):
-            word = self.status.tolist()
+        word = [] if self.status is None else self.status.tolist()
+        if any(word[::8]):
             self.status.zero_()          # each report is raised once, and says nothing about later calls
             if self._seen is not None:
                 self._seen.zero_()       # (its copies are done: the read above waited for them)
             raise KernelError(f"device status {word}")
+
+    def _word(self, i: int) -> Optional[torch.Tensor]:
+        """Error word 0, for the kernels that report bad places and go on, or 1, for the prefill attention: it
+        gives up its waits, with copies in flight, once its word is set, so only its own reports may set it."""
+        return None if self.status is None else self.status[8 * i:8 * i + 8]
 
     def _look(self) -> None:
         if self._seen is not None:
             self._seen.copy_(self.status, non_blocking=True)
 
     def _raise_seen(self) -> None:
-        if self._seen is not None and int(self._seen[0]):
+        if self._seen is not None and any(self._seen[::8].tolist()):
             self.check_device()
 
     @torch.no_grad()
@@ -232,16 +238,16 @@ class _Step:
         plan = c.plan(self.add, self.n, out=self.plan)
         planned()
         x = self.x
-        x.copy_(K.embedding(self.tokens, w.embed, status=d.status))
+        x.copy_(K.embedding(self.tokens, w.embed, status=d._word(0)))
         for li, lw in enumerate(w.layers):
             if few:
                 qkv = K.gemv(x, lw.wqkv, "f32", bias=lw.bqkv, y_f32=self.qkv, norm_w=lw.in_norm, eps=eps)
             else:
                 qkv = K.gemm(K.rmsnorm(x, lw.in_norm, eps), lw.wqkv, "bias" if lw.bqkv is not None else "store", bias=lw.bqkv)
             paged.rope_append_kv8(qkv, d.cos, d.sin, plan.pos, plan.unit, c.block_table, *c.layer(li), heads=d.H,
-                                  q_out=self.q, status=d.status)
+                                  q_out=self.q, status=d._word(0))
             paged.attention_kv8(self.q, *c.layer(li), c.block_table, c.kv_len, plan.cu, max_q=1, scale=d.scale, out=self.o,
-                                want_lse=False, status=d.status)
+                                want_lse=False, status=d._word(0))
             o = self.o.view(self.n, -1)
             if few:
                 K.gemv(o, lw.wo, "residual", y_bf16=x)

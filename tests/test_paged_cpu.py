@@ -425,6 +425,32 @@ def test_generate_raises_for_a_report_and_clears_it():
     assert torch.equal(dec.generate([torch.arange(5)], 3)[0], want)
 
 
+def test_prefill_attention_has_an_error_word_of_its_own(monkeypatch):
+    """A report of another kernel (a token id, a position) must not end the waits of the prefill attention."""
+    from hetero_cp_ringattn_b200.models import paged as model
+    dec = _small_decoder()
+    dec.status = torch.zeros(16, dtype=torch.int32)
+    words = {"append": [], "attention": []}
+
+    def spy(name, fn):
+        def call(*a, status=None, **k):
+            words[name].append(status.data_ptr())
+            return fn(*a, **k)
+        return call
+
+    monkeypatch.setattr(paged, "rope_append_kv8", spy("append", paged.rope_append_kv8))
+    monkeypatch.setattr(model.K, "attention", spy("attention", model.K.attention))
+    dec.prefill(0, torch.arange(20), piece=16)
+    assert len(words["append"]) == len(words["attention"]) == 2 * dec.cfg.num_layers
+    assert len(set(words["append"])) == len(set(words["attention"])) == 1
+    assert abs(words["append"][0] - words["attention"][0]) >= 16
+    for i in (0, 8):
+        dec.status[i] = 16
+        with pytest.raises(KernelError):
+            dec.check_device()
+        dec.check_device()
+
+
 def test_generate_leaves_rows_in_use_alone():
     """A session in row 0: prompts take other rows, and are refused where those do not suffice."""
     dec, alone = _small_decoder(), _small_decoder()
